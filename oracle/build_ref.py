@@ -50,7 +50,7 @@ MODULES = {
 
 def build(ref_root=REF_ROOT, force=False):
     """Returns the list of cubins built or already present; [] when the reference is absent."""
-    if not os.path.isdir(ref_root):
+    if not os.path.isdir(os.path.join(ref_root, "source")):
         return [os.path.join(OUT, f) for f in sorted(os.listdir(OUT))] if os.path.isdir(OUT) else []
     os.makedirs(OUT, exist_ok=True)
     done = []

@@ -32,6 +32,7 @@ extern "C" {
 #define K3G_EALIGN (-3) /* pointer not 16-byte aligned */
 #define K3G_ERANGE (-4) /* rank / slot / nb / order out of range */
 #define K3G_ELIMIT (-5) /* size beyond a built-in maximum */
+#define K3G_EWORKSPACE (-6) /* workspace smaller than the call needs */
 
 /* ---- residual stream --------------------------------------------------------------------- */
 
@@ -385,6 +386,57 @@ int k3g_span_state(void* kda_base, const void* line_index, long long line_bytes,
  * contiguous from 64-row pages; rows >= lens[0] are zero. */
 int k3g_latent_gather(const void* slab, const void* block_table, long long page_stride, const void* lens, void* out, int n,
                       void* stream);
+
+/* ---- decoding with drafts over the latent cache (no counterpart in the reference, which only prefills) ---------- */
+/* The cache is paged as k3g_mla_prep writes it: pages of 64 tokens, a page table per sequence, `layer_off` the layer's place in
+ * a page.  bf16 pages are 64 rows of 576 (512 latent columns, 64 rope columns); offsets and strides in elements.  MXFP8 pages
+ * are 41984 bytes in three planes -- 64 x 512 E4M3 codes, 64 x 64 bf16 (the rope columns as they are), 64 x 16 UE8M0 scale bytes --
+ * 656 bytes a token instead of 1152; offsets and strides in bytes, multiples of 16.  `pages` is the number of pages the cache
+ * holds: a table entry outside [0, pages) is never read, and neither is one behind the last token of its sequence. */
+
+/* Quantise T latent rows (576 bf16, `row_stride` elements apart, a multiple of 8) and append them: row t goes to slot
+ * slot_mapping[t] (i64: page * 64 + row; a slot outside [0, 64 * pages) is skipped).  Codes and scales are k3g_moe_quant's for the
+ * same values.  The slots of one call have to differ: of two rows with one slot parts of either may stay. */
+int k3g_latent_mx8_store(const void* rows, long long row_stride, const void* slot_mapping, void* cache, long long layer_off,
+                         long long page_stride, long long pages, int T, void* stream);
+
+/* k3g_latent_gather for MXFP8 pages: out [n, 576] bf16 = the tokens of block_table (i32) in order, code * 2^(scale - 127)
+ * exactly; rows from lens[0] (i32) on, and rows of pages outside [0, pages), are zero. */
+int k3g_latent_mx8_gather(const void* cache, const void* block_table, long long layer_off, long long page_stride, long long pages,
+                          const void* lens, void* out, int n, void* stream);
+
+/* Attention of a batch over the cache, a prefix that all its sequences share read once for all of them:
+ *   out[b, s, h] [512] = sum_j p_j k_j[0:512],  p = softmax_j(scale * q[b, s, h] . k_j)   (k_j: 576 columns of token j)
+ * over the first prefix_len[0] tokens of prefix_table [prefix_pages], which every row sees, and the first
+ * lens[b] - (S - 1 - s) tokens of block_table[b] [B, max_pages]: the last S of a sequence's own tokens are its S steps (S = 1 plain
+ * decoding, S > 1 drafted tokens), whose latents are in the cache before the call.  All i32 on the device; lengths beyond the
+ * tables' capacity are cut to it.  q [B, S, heads, 576] bf16, q_stride elements (a multiple of 8) from one step to the next; out
+ * [B, S, heads, 512] bf16.
+ *   - lens[b] < 0: no sequence (a padded batch); its rows of out are left as they were.
+ *   - a row that sees no token is zero; one that sees a NaN or an infinity is NaN, the others are not touched by it; what lies
+ *     behind the last token of a page is not used.
+ *   - prefix_pages = 0 / max_pages = 0: no prefix / no own tokens (the tables, and prefix_len, may be null).
+ *   - workspace: 16-byte aligned device memory of k3g_latent_attn_workspace bytes (else K3G_EWORKSPACE), used by one call at a time:
+ *     calls that may overlap, and captured graphs that may run together, need one each.  Its content need not be kept.
+ * B <= 4096, S * heads <= 32768, prefix_pages and max_pages <= 2^20 (K3G_ELIMIT). */
+int k3g_latent_attn(const void* q, long long q_stride, const void* cache, int cache_mx8, long long layer_off, long long page_stride,
+                    long long pages, const void* prefix_table, const void* prefix_len, int prefix_pages, const void* block_table,
+                    const void* lens, int max_pages, void* out, void* workspace, long long workspace_bytes, int B, int S, int heads,
+                    float scale, void* stream);
+/* Workspace of k3g_latent_attn for a batch of at most this shape: *host_bytes, a host address.  Launches nothing. */
+int k3g_latent_attn_workspace(int B, int S, int heads, long long* host_bytes);
+
+/* Verification of drafted tokens by rejection sampling, from given random numbers.  target [B, S + 1, V] f32: the target's
+ * probabilities after each of 0 .. S drafts (rows target_stride elements apart); draft [B, S, V] f32: the draft model's (rows
+ * draft_stride apart), or null for drafts without probabilities (greedy or looked up: 1 at the draft); ids [B, S] i64 the drafts;
+ * u [B, S + 1] f32 in [0, 1).  Draft i is kept while u[b, i] * q_i(ids[b, i]) < p_i(ids[b, i]); an id outside [0, V) ends the
+ * sequence's drafts.  One more token follows the kept ones: at a draft turned down the first v whose running sum of max(p - q, 0)
+ * exceeds u[b, S] times the whole sum, else (all kept, or p <= q everywhere) the same of p; sums in 64 bits, rows need not be
+ * normalised, NaN, negative and infinite weights count as 0.  accepted [B] i32 = drafts kept; tokens [B, S + 1] i64 = the kept drafts, the token
+ * that follows (-1 if its row weighs nothing), then -1.  S <= 32, V <= 2^30, B <= 2^24.  Rows with strides that are multiples of 4 are
+ * read 16 bytes at a time. */
+int k3g_verify_draft(const void* target, long long target_stride, const void* draft, long long draft_stride, const void* ids, const void* u,
+                     void* accepted, void* tokens, int B, int S, int V, void* stream);
 
 #ifdef __cplusplus
 }

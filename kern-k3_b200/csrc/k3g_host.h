@@ -15,6 +15,7 @@
 #define K3G_EALIGN (-3)   /* a pointer is not 16-byte aligned */
 #define K3G_ERANGE (-4)   /* an index argument is out of range (rank, slot, nb, order) */
 #define K3G_ELIMIT (-5)   /* a size exceeds a built-in maximum */
+#define K3G_EWORKSPACE (-6) /* a workspace is smaller than the call needs */
 
 #define K3G_API extern "C" __attribute__((visibility("default")))
 

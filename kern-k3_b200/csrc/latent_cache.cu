@@ -1,0 +1,101 @@
+// MXFP8 latent cache: rows quantised as they are appended, and pages read back as contiguous bf16 rows.
+//
+// For a row x of 576 bf16 and each block of 32 of its first 512 columns: e = the smallest integer with 448 * 2^e >= max|x|
+// (0 for an all-zero block), code = E4M3(x * 2^-e) to nearest even, scale byte e + 127; the last 64 columns stay bf16.
+// Reading back gives code * 2^e, which bf16 holds exactly.  No counterpart in the reference, whose cache is bf16
+// (source/k3_mla_prep_v2.cu:200-211 writes it, source/k3_mla_v2.cu:22-33 reads it).
+//
+// Bound by HBM: 1808 bytes a row either way.  ONE WARP PER ROW: lane l owns columns 16 l .. 16 l + 15, so a block of 32 is
+// two neighbouring lanes (its maximum is one shuffle), codes move as one 16-byte access per lane, and lanes 0..7 move the
+// rope columns.  No shared memory, no block barrier.
+#include "latent_page.cuh"
+#include "k3g_host.h"
+
+using namespace k3g;
+
+namespace {
+
+constexpr int kWarps = 8;
+
+__global__ void __launch_bounds__(32 * kWarps) latent_mx8_store_kernel(const __nv_bfloat16* __restrict__ rows, long long row_stride,
+                                                                       const long long* __restrict__ slot_mapping,
+                                                                       unsigned char* __restrict__ cache, long long page_stride,
+                                                                       long long slots, int T) {
+  const int lane = threadIdx.x & 31;
+  for (int t = blockIdx.x * kWarps + (threadIdx.x >> 5); t < T; t += gridDim.x * kWarps) {
+    const __nv_bfloat16* row = rows + t * row_stride;
+    const V8 a = ld_stream(row + 16 * lane), b = ld_stream(row + 16 * lane + 8);
+    V8 r;
+    if (lane < 8) r = ld_stream(row + kLatent + 8 * lane);
+    const long long slot = __ldg(slot_mapping + t);
+    unsigned m = max_bf16_bits(absmax8(a), absmax8(b));
+    m = max_bf16_bits(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    const int e = ue8m0_exp_from_bf16(m);
+    const float s = pow2_neg(e);
+    V8 q;
+    quant8(a, s, q.w[0], q.w[1]);
+    quant8(b, s, q.w[2], q.w[3]);
+    if (slot < 0 || slot >= slots) continue;                 // no slot: nothing is appended
+    unsigned char* page = cache + (slot >> 6) * page_stride;
+    const int at = (int)(slot & 63);
+    st_plain(page + at * kLatent + 16 * lane, q);
+    if (lane < 8) st_plain(page + kPageRope + at * (2 * kRopeCols) + 16 * lane, r);
+    if ((lane & 1) == 0) page[kPageScales + at * (kLatent / 32) + (lane >> 1)] = (unsigned char)(e + 127);
+  }
+}
+
+__global__ void __launch_bounds__(32 * kWarps) latent_mx8_gather_kernel(const unsigned char* __restrict__ cache, const int* __restrict__ block_table,
+                                                                        long long page_stride, long long pages, const int* __restrict__ lens,
+                                                                        __nv_bfloat16* __restrict__ out, int n) {
+  const int lane = threadIdx.x & 31;
+  const int len = lens[0];
+  for (int t = blockIdx.x * kWarps + (threadIdx.x >> 5); t < n; t += gridDim.x * kWarps) {
+    V8 a = {{0u, 0u, 0u, 0u}}, b = a, r = a;
+    if (t < len) {
+      const int id = __ldg(block_table + (t >> 6));
+      if (id >= 0 && id < pages) {
+        const unsigned char* page = cache + id * page_stride;
+        const int at = t & 63;
+        const V8 q = ld_stream(page + at * kLatent + 16 * lane);
+        if (lane < 8) r = ld_stream(page + kPageRope + at * (2 * kRopeCols) + 16 * lane);
+        const float s = ue8m0_value(__ldg(page + kPageScales + at * (kLatent / 32) + (lane >> 1)));
+        mx8_to_bf16x4(q.w[0], s, a.w[0], a.w[1]);
+        mx8_to_bf16x4(q.w[1], s, a.w[2], a.w[3]);
+        mx8_to_bf16x4(q.w[2], s, b.w[0], b.w[1]);
+        mx8_to_bf16x4(q.w[3], s, b.w[2], b.w[3]);
+      }
+    }
+    __nv_bfloat16* row = out + (long long)t * kRow;
+    st_stream(row + 16 * lane, a);
+    st_stream(row + 16 * lane + 8, b);
+    if (lane < 8) st_stream(row + kLatent + 8 * lane, r);
+  }
+}
+
+}  // namespace
+
+K3G_API int k3g_latent_mx8_store(const void* rows, long long row_stride, const void* slot_mapping, void* cache, long long layer_off,
+                                 long long page_stride, long long pages, int T, void* stream) {
+  K3G_REQUIRE_PTR(rows); K3G_REQUIRE_PTR(slot_mapping); K3G_REQUIRE_PTR(cache);
+  K3G_REQUIRE_ALIGNED(rows); K3G_REQUIRE_ALIGNED(cache);
+  K3G_REQUIRE(row_stride % 8 == 0 && layer_off % 16 == 0 && page_stride % 16 == 0, K3G_EALIGN);
+  K3G_REQUIRE(T >= 0 && pages >= 0 && pages < (1ll << 31), K3G_ESHAPE);
+  if (T == 0) return K3G_OK;
+  K3G_REQUIRE(row_stride >= kRow && layer_off >= 0 && page_stride >= layer_off + kMx8Page, K3G_ESHAPE);
+  latent_mx8_store_kernel<<<(T - 1) / kWarps + 1, 32 * kWarps, 0, k3g_stream(stream)>>>(
+      (const __nv_bfloat16*)rows, row_stride, (const long long*)slot_mapping, (unsigned char*)cache + layer_off, page_stride, pages * kPageTokens, T);
+  return k3g_launch_status();
+}
+
+K3G_API int k3g_latent_mx8_gather(const void* cache, const void* block_table, long long layer_off, long long page_stride, long long pages,
+                                  const void* lens, void* out, int n, void* stream) {
+  K3G_REQUIRE_PTR(cache); K3G_REQUIRE_PTR(block_table); K3G_REQUIRE_PTR(lens); K3G_REQUIRE_PTR(out);
+  K3G_REQUIRE_ALIGNED(cache); K3G_REQUIRE_ALIGNED(out);
+  K3G_REQUIRE(layer_off % 16 == 0 && page_stride % 16 == 0, K3G_EALIGN);
+  K3G_REQUIRE(n >= 0 && pages >= 0 && pages < (1ll << 31), K3G_ESHAPE);
+  if (n == 0) return K3G_OK;
+  K3G_REQUIRE(layer_off >= 0 && page_stride >= layer_off + kMx8Page, K3G_ESHAPE);
+  latent_mx8_gather_kernel<<<(n - 1) / kWarps + 1, 32 * kWarps, 0, k3g_stream(stream)>>>(
+      (const unsigned char*)cache + layer_off, (const int*)block_table, page_stride, pages, (const int*)lens, (__nv_bfloat16*)out, n);
+  return k3g_launch_status();
+}

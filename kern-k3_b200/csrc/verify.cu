@@ -1,0 +1,217 @@
+// Verification of drafted tokens by rejection sampling, from given random numbers.
+//
+// For each sequence: draft i (token x) is kept while u_i * q_i(x) < p_i(x), p the target's probabilities and q the draft
+// model's (1 at x for drafts without probabilities); the products are exact in 64 bits.  At the first draft turned down
+// one more token is drawn from max(p - q, 0), and from p when every draft was kept, or when p <= q everywhere: the first v with
+// sum_{w <= v} weight(w) > u * sum(weight).  Sums are 64-bit: a token is decided by where u falls between neighbouring
+// sums of up to 10^5 terms, which 32 bits place wrongly about once in a hundred draws.  No atomics: every sum has a fixed order.
+//
+// Bound by HBM: one row of p and one of q per sequence (the other rows are touched at one entry each).  ONE CLUSTER PER
+// SEQUENCE, in one launch and without a workspace: each block sums a slice of the row, one contiguous segment per warp,
+// the segment sums are exchanged through distributed shared memory, and the one warp whose segment holds the drawn point
+// reads its segment again (from L2) and finds the token.
+#include <cooperative_groups.h>
+
+#include "k3g_device.cuh"
+#include "k3g_host.h"
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+constexpr int kThreads = 512, kSegs = kThreads / 32, kMaxCluster = 8, kMaxSteps = 32;
+
+struct Rows {                       // the row that is sampled from: weight(v) = p[v], or max(p[v] - q(v), 0)
+  const float* p;
+  const float* q;                   // null: q is 1 at `hot` and 0 elsewhere (hot < 0: 0 everywhere, the weight is p)
+  int hot;
+};
+__device__ __forceinline__ double weight(float p, float q) {
+  const double d = (double)p - (double)q;
+  return d > 0.0 && d < (double)INFINITY ? d : 0.0;          // NaN and infinite entries weigh nothing
+}
+__device__ __forceinline__ float q_at(const Rows& r, int v) { return r.q ? __ldg(r.q + v) : (v == r.hot ? 1.f : 0.f); }
+
+// Weights of elements v .. v + 3 (those below `end`).
+template <bool VEC>
+__device__ __forceinline__ void weights4(const Rows& r, int v, int end, double (&w)[4]) {
+  float p[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
+  if (VEC && v + 4 <= end) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(r.p + v));
+    p[0] = a.x; p[1] = a.y; p[2] = a.z; p[3] = a.w;
+    if (r.q) {
+      const float4 b = __ldg(reinterpret_cast<const float4*>(r.q + v));
+      q[0] = b.x; q[1] = b.y; q[2] = b.z; q[3] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j] = v + j == r.hot ? 1.f : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (v + j < end) { p[j] = __ldg(r.p + v + j); q[j] = q_at(r, v + j); }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = weight(p[j], q[j]);
+}
+
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+__device__ __forceinline__ double lane_scan(double x, int lane) {   // sum of the lanes up to and including this one
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+template <bool VEC>
+__device__ __forceinline__ double segment_sum(const Rows& r, int lo, int hi, int lane) {
+  double s = 0.0;
+#pragma unroll 4
+  for (int v = lo + 4 * lane; v < hi; v += 128) {
+    double w[4];
+    weights4<VEC>(r, v, hi, w);
+    s += (w[0] + w[1]) + (w[2] + w[3]);
+  }
+  return warp_sum(s);
+}
+
+// First element of [lo, hi) whose running sum, on top of `base`, passes `point`; the last one with a weight if rounding
+// keeps the sums below it; -1 if no element weighs anything.
+template <bool VEC>
+__device__ __forceinline__ int segment_find(const Rows& r, int lo, int hi, double base, double point, int lane) {
+  int last = -1;
+  for (int v0 = lo; v0 < hi; v0 += 128) {
+    const int v = v0 + 4 * lane;
+    double w[4] = {0.0, 0.0, 0.0, 0.0};
+    if (v < hi) weights4<VEC>(r, v, hi, w);
+    const double mine = (w[0] + w[1]) + (w[2] + w[3]);
+    const double upto = lane_scan(mine, lane);
+    double c = __shfl_up_sync(0xffffffffu, upto, 1);
+    c = base + (lane == 0 ? 0.0 : c);
+    int hit = -1, top = -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c += w[j];
+      if (w[j] > 0.0) { top = v + j; if (hit < 0 && c > point) hit = v + j; }
+    }
+    const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0);
+    if (hits) return __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+    const unsigned tops = __ballot_sync(0xffffffffu, top >= 0);
+    if (tops) last = __shfl_sync(0xffffffffu, top, 31 - __clz(tops));
+    base += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return last;
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(kThreads) verify_draft_kernel(const float* __restrict__ target, long long target_stride,
+                                                                const float* __restrict__ draft, long long draft_stride,
+                                                                const long long* __restrict__ ids, const float* __restrict__ u,
+                                                                int* __restrict__ accepted, long long* __restrict__ tokens, int S, int V,
+                                                                int slice) {
+  __shared__ double s_sum[kSegs];
+  __shared__ double s_all[kMaxCluster * kSegs];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.x / ranks;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+
+  // every warp decides for itself which drafts stay
+  bool valid = false, keep = false;
+  if (lane < S) {
+    const long long x = ids[(long long)b * S + lane];
+    valid = x >= 0 && x < V;
+    if (valid) {
+      const double px = target[((long long)b * (S + 1) + lane) * target_stride + x];
+      const double qx = draft ? (double)draft[((long long)b * S + lane) * draft_stride + x] : 1.0;
+      keep = (double)u[(long long)b * (S + 1) + lane] * qx < px;
+    }
+  }
+  const unsigned kept_mask = __ballot_sync(0xffffffffu, valid && keep), valid_mask = __ballot_sync(0xffffffffu, valid);
+  const int kept = __ffs(~kept_mask) ? min(__ffs(~kept_mask) - 1, S) : S;
+  const bool turned_down = kept < S && ((valid_mask >> kept) & 1u);
+  Rows r;
+  r.p = target + ((long long)b * (S + 1) + kept) * target_stride;
+  r.q = turned_down && draft ? draft + ((long long)b * S + kept) * draft_stride : nullptr;
+  r.hot = turned_down && !draft ? (int)ids[(long long)b * S + kept] : -1;
+
+  // the slice of this block, one contiguous segment (a multiple of 4 elements) for each warp
+  const int seg = (slice / kSegs);
+  const int lo = min(V, (rank * kSegs + warp) * seg), hi = min(V, lo + seg);
+  double total = 0.0, upto = 0.0, part[4];                   // lane l looks after segments 4 l .. 4 l + 3
+  for (int pass = 0; pass < 2; ++pass) {
+    const double mine = segment_sum<VEC>(r, lo, hi, lane);
+    if (lane == 0) s_sum[warp] = mine;
+    cluster.sync();
+    if (threadIdx.x < ranks * kSegs) s_all[threadIdx.x] = cluster.map_shared_rank(s_sum, threadIdx.x / kSegs)[threadIdx.x % kSegs];
+    cluster.sync();                                          // read by all before any block goes on (or ends)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[j] = 4 * lane + j < ranks * kSegs ? s_all[4 * lane + j] : 0.0;
+    upto = lane_scan((part[0] + part[1]) + (part[2] + part[3]), lane);
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    if (total > 0.0 || (!r.q && r.hot < 0)) break;
+    r.q = nullptr; r.hot = -1;                               // p <= q everywhere: draw from p
+  }
+  // the segment that holds the point: the first whose running sum passes it, else the last that weighs anything
+  const double point = (double)u[(long long)b * (S + 1) + S] * total;
+  double base = __shfl_up_sync(0xffffffffu, upto, 1);
+  if (lane == 0) base = 0.0;
+  int hit = -1, top = -1;
+  double hit_base = 0.0, top_base = 0.0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (part[j] > 0.0) {
+      top = 4 * lane + j; top_base = base;
+      if (hit < 0 && base + part[j] > point) { hit = top; hit_base = base; }
+    }
+    base += part[j];
+  }
+  const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), tops = __ballot_sync(0xffffffffu, top >= 0);
+  const int from = hits ? __ffs(hits) - 1 : tops ? 31 - __clz(tops) : 0;
+  const int pick_seg = __shfl_sync(0xffffffffu, hits ? hit : top, from);
+  base = __shfl_sync(0xffffffffu, hits ? hit_base : top_base, from);
+  if (pick_seg < 0 ? (rank == 0 && warp == 0) : pick_seg == rank * kSegs + warp) {
+    const int pick = pick_seg < 0 ? -1 : segment_find<VEC>(r, lo, hi, base, point, lane);
+    if (lane == 0) accepted[b] = kept;
+    for (int i = lane; i <= S; i += 32)
+      tokens[(long long)b * (S + 1) + i] = i < kept ? ids[(long long)b * S + i] : i == kept ? (long long)pick : -1ll;
+  }
+}
+
+}  // namespace
+
+K3G_API int k3g_verify_draft(const void* target, long long target_stride, const void* draft, long long draft_stride, const void* ids, const void* u,
+                             void* accepted, void* tokens, int B, int S, int V, void* stream) {
+  K3G_REQUIRE_PTR(target); K3G_REQUIRE_PTR(ids); K3G_REQUIRE_PTR(u); K3G_REQUIRE_PTR(accepted); K3G_REQUIRE_PTR(tokens);
+  K3G_REQUIRE_ALIGNED(target); if (draft) K3G_REQUIRE_ALIGNED(draft);
+  K3G_REQUIRE(B >= 0 && S >= 0 && V >= 0, K3G_ESHAPE);
+  K3G_REQUIRE(S <= kMaxSteps && B <= (1 << 24) && V <= (1 << 30), K3G_ELIMIT);
+  if (B == 0) return K3G_OK;
+  K3G_REQUIRE(V > 0 && target_stride >= V && (!draft || draft_stride >= V), K3G_ESHAPE);
+  // Blocks per sequence: as many as fit the card in one wave (four blocks of 512 threads on each of 148 SMs), while a block
+  // still has a few thousand elements to read.
+  int ranks = kMaxCluster;
+  while (ranks > 1 && ((long long)B * ranks > 592 || V < ranks * 2048)) ranks /= 2;
+  const int per = kSegs * 4 * ranks;
+  const int slice = (int)(((long long)V + per - 1) / per) * kSegs * 4;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(B * ranks), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.stream = k3g_stream(stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)ranks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cfg.attrs = at; cfg.numAttrs = 1;
+  const bool vec = target_stride % 4 == 0 && (!draft || draft_stride % 4 == 0);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, vec ? verify_draft_kernel<true> : verify_draft_kernel<false>, (const float*)target, target_stride,
+                                           (const float*)draft, draft_stride, (const long long*)ids, (const float*)u, (int*)accepted,
+                                           (long long*)tokens, S, V, slice);
+  if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
+  return k3g_launch_status();
+}

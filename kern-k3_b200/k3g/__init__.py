@@ -18,7 +18,7 @@ CUBIN_DIR = os.path.join(_ROOT, "lib", "cubin")
 
 ERRORS = {-1: "K3G_ENULL: a required pointer is null", -2: "K3G_ESHAPE: unsupported size",
           -3: "K3G_EALIGN: pointer not 16-byte aligned", -4: "K3G_ERANGE: index argument out of range",
-          -5: "K3G_ELIMIT: size beyond a built-in maximum"}
+          -5: "K3G_ELIMIT: size beyond a built-in maximum", -6: "K3G_EWORKSPACE: workspace smaller than the call needs"}
 
 
 class K3gError(RuntimeError):
@@ -103,3 +103,10 @@ def call(name, *args):
 def current_stream():
     import torch
     return torch.cuda.current_stream().cuda_stream
+
+
+def latent_attn_workspace(B, S, heads):
+    """Bytes of workspace k3g_latent_attn needs for a batch of at most this shape."""
+    n = ctypes.c_longlong()
+    call("k3g_latent_attn_workspace", B, S, heads, n)
+    return n.value

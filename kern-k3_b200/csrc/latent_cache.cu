@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(32 * kWarps) latent_mx8_gather_kernel(const un
         const int at = t & 63;
         const V8 q = ld_stream(page + at * kLatent + 16 * lane);
         if (lane < 8) r = ld_stream(page + kPageRope + at * (2 * kRopeCols) + 16 * lane);
-        const float s = ue8m0_value(__ldg(page + kPageScales + at * (kLatent / 32) + (lane >> 1)));
+        const unsigned s = ue8m0_pair(__ldg(page + kPageScales + at * (kLatent / 32) + (lane >> 1)));
         mx8_to_bf16x4(q.w[0], s, a.w[0], a.w[1]);
         mx8_to_bf16x4(q.w[1], s, a.w[2], a.w[3]);
         mx8_to_bf16x4(q.w[2], s, b.w[0], b.w[1]);

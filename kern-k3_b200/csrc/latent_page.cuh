@@ -17,19 +17,17 @@ constexpr int kPageRope = kPageTokens * kLatent, kPageScales = kPageRope + kPage
 constexpr int kMx8Page = kPageScales + kPageTokens * (kLatent / 32);                          // 41984 bytes
 constexpr int kBf16Page = kPageTokens * kRow;                                                 // 36864 elements
 
-// 2^(s - 127); 255 is the format's NaN, 0 the subnormal 2^-127.
-__device__ __forceinline__ float ue8m0_value(unsigned s) {
-  return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fffffffu : s << 23);
-}
+// 2^(s - 127) as a pair of bf16: 0 is the subnormal 2^-127, 255 the format's NaN.
+__device__ __forceinline__ unsigned ue8m0_pair(unsigned s) { return (s == 0 ? 0x0040u : s == 255 ? 0x7fffu : s << 7) * 0x10001u; }
 
-// Four E4M3 codes times a power of two -> four bf16 in two words.  A code has four significant bits, so the product is
-// exact in f32 and in bf16 (but for the last bits of bf16 subnormals).
-__device__ __forceinline__ void mx8_to_bf16x4(unsigned codes, float scale, unsigned& lo, unsigned& hi) {
+// Four E4M3 codes times a power of two -> four bf16 in two words.  A code has four significant bits, so it is exact in f16 (which the
+// conversion gives) and in bf16, and so is its product (but for the last bits of bf16 subnormals, rounded once).
+__device__ __forceinline__ void mx8_to_bf16x4(unsigned codes, unsigned scale, unsigned& lo, unsigned& hi) {
   unsigned h0, h1;
   asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b;}" : "=r"(h0), "=r"(h1) : "r"(codes));
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-  lo = pack_bf2(__fmul_rn(a.x, scale), __fmul_rn(a.y, scale));
-  hi = pack_bf2(__fmul_rn(b.x, scale), __fmul_rn(b.y, scale));
+  lo = mul_bf2(pack_bf2(a.x, a.y), scale);
+  hi = mul_bf2(pack_bf2(b.x, b.y), scale);
 }
 
 }  // namespace k3g

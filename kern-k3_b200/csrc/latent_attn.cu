@@ -12,16 +12,17 @@
 // sum in 32 bits), and a second, dependent launch joins the parts of each row.  Lengths and tables are read on the device:
 // a captured graph follows them.  Nothing is accumulated by atomics: the same inputs give the same bits.
 //
-// One CTA per SM, warps with fixed roles, one tile after another:
-//   8 softmax warps  S from tensor memory, running maximum, P = 2^(S - m) rounded to 16 bits into shared memory; O scaled, read and written out;
-//   16 loader warps  fetch the next tile's codes into registers and make 16-bit floats of them in 128-byte-swizzled shared memory, in nine
-//                    16 KB chunks of 64 columns;
+// One CTA per SM, warps with fixed roles, one token tile after another:
 //   1 planning warp  this CTA's stretches, one after another, into a ring that the others read;
-//   1 MMA warp       S = Q K^T (64 x 128, chunk by chunk as they come) and O += P V (64 x 512 in tensor memory), both tcgen05.mma.ws, M = 64.
+//   16 loader warps  fetch the next tile into registers and make 16-bit floats of it in 128-byte-swizzled shared memory, nine 16 KB chunks of 64
+//                    columns;
+//   1 MMA warp       S = Q K^T (64 x 128, two chunks at a time as they come) and O += P V (64 x 512 in tensor memory), both tcgen05.mma.ws, M = 64;
+//   8 softmax warps  S from tensor memory, running maximum, P = 2^(S - m) rounded to 16 bits into shared memory; O scaled, read and written out.
 // Why M = 64: a 128-row O of 512 columns fills the whole tensor memory and leaves no room for S.  The weight-stationary form puts
 // a 64-row tile on all 128 lanes and reaches 48 cycles per 64 x 128 x 16 step, the plain form 64 (measured; 32 would be full rate).
-// Why 128 tokens: the 64 x 64 x 16 step of S costs 44 cycles.  Why O in four products of 128 columns: the slots of a pair of chunks
-// are free for the next tile after a quarter of P V.  The queries' rope columns lie in tensor memory, which makes room for P.
+// Why 128 tokens: a 64 x 64 x 16 step costs 44 cycles.  What bounds a tile is shared memory (operands of both products, the loaders' stores: 0.5 MB), so
+// pages of 64 tokens in two buffers, which let all roles work at once, took longer (2.3 against x us a tile).  O is made in four products of 128
+// columns: a pair of chunks is refilled as soon as its quarter of P V is done.  The queries' rope columns lie in tensor memory, which makes room for P.
 //
 // Types.  bf16 pages are multiplied as bf16.  MXFP8 codes become f16, not bf16: one conversion and one product for two codes, a third of what bf16
 // takes (which has no conversion from E4M3), and the loaders' instructions are what a tile waits for.  f16 has the bits (a code has four), but not the
@@ -41,12 +42,11 @@ using namespace k3g;
 namespace {
 
 constexpr int kMaxBatch = 4096, kMaxRowsPerSeq = 1 << 15, kMaxCtas = 160;
-constexpr int kRows = 64, kTile = 128;                       // query rows and tokens of a tile
+constexpr int kRows = 64, kTile = 2 * kPageTokens;           // query rows and tokens of a tile
 constexpr int kSoftmax = 256, kLoaders = 512, kThreads = kSoftmax + kLoaders + 128;   // the last four warps: MMAs, planning, two idle
-constexpr int kChunk = kTile * 128;                          // 64 columns of a tile's tokens, bf16
-constexpr int kQChunk = kRows * 128;
+constexpr int kChunk = kTile * 128, kQChunk = kRows * 128;   // 64 columns of a tile's tokens, of its rows, at 16 bits
 constexpr int kSmemQ = 8 * kQChunk, kSmemP = 2 * kQChunk, kSmemK = 9 * kChunk, kSmem = kSmemQ + kSmemP + kSmemK + 1024;
-// tensor memory columns: O 0..255 (four accumulators of 128 output columns, 64 on either half of the lanes), S 256..319 (64 tokens on either
+// tensor memory columns: O 0..255 (four accumulators of 128 output columns, 64 on either half of the lanes), S 256..319 (a page on either
 // half), the rope columns' part of S 320..383 (MXFP8), the queries' rope columns 384..415 (the same on both halves)
 constexpr int kTmemS = 256, kTmemR = 320, kTmemQ = 384;
 constexpr int kLeastE = -80, kMostE = 120;                   // exponents of 8 tokens: sums of 2^-E stay in range
@@ -92,28 +92,35 @@ struct Segment {                     // one CTA's stretch of one row tile
 
 // ---- barriers and tensor memory -----------------------------------------------------------------------------------------------
 struct Control {
-  unsigned long long full[5], empty[4], q_full, s_full, p_full[2];
+  unsigned long long full[5], empty[4], s_full, p_full, q_full, o_free;
   unsigned long long ring_full[kRing], ring_empty[kRing];
   Segment ring[kRing];
   unsigned tmem;
   int abort;
   int first_tile, first_at;
-  long long scan[kThreads / 32], left;
-  unsigned poison[2][4];
-  int exponent[2][16];                                        // E of each 8 tokens of a tile
-  float row_scale[kRows];                                     // 2^(what was taken out of a query row)
-  float best[4][kRows];                                      // the maxima of a tile, and at a segment's end the sums
+  long long left;
+  unsigned poison[2][4];                                      // tokens of a tile with values that are not finite (tiles by turns)
+  alignas(16) int exponent[16];
+  int tokens[2];                                // of a tile: E of each 8 tokens, and how many there are in either page
+  float row_scale[2][kRows];                                  // 2^(what was taken out of a query row), segments by turns
+  union {
+    float best[4][kRows];                                     // the maxima of a page, and at a segment's end the sums
+    long long scan[kThreads / 32];                            // before the first
+  };
 };
 
 // Every wait ends: after kWaitLimit polls, or as soon as another wait of the CTA has expired.  The roles then run through what is
 // left without waiting (every access stays where it was), and the call's result is NaN.
-__device__ __forceinline__ void wait(Control& k, unsigned long long& bar, unsigned parity) {
+__device__ __forceinline__ void wait(Control& k, unsigned long long& bar, unsigned parity, unsigned nap = 0) {
+  unsigned ok;
+  asm volatile("{.reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}" : "=r"(ok) : "r"(su(&bar)), "r"(parity) : "memory");
+  if (ok) return;
 #pragma unroll 1
   for (int i = 0; i < kWaitLimit; ++i) {
-    unsigned ok;
     asm volatile("{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}" : "=r"(ok) : "r"(su(&bar)), "r"(parity) : "memory");
     if (ok) return;
     if (*(volatile int*)&k.abort) return;
+    if (nap) __nanosleep(nap);
   }
   *(volatile int*)&k.abort = 1;
 }
@@ -168,8 +175,8 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // ---- loaders ----------------------------------------------------------------------------------------------------------------------
-// Warp w looks after tokens 8 w .. 8 w + 7 of a tile, in two steps j of four tokens (token 8 w + 4 j + lane / 8), eight lanes to a token:
-// an access of the warp is four runs of 128 bytes.
+// Warp w looks after tokens 8 w .. + 7 of a tile, lane x after token 8 w + x % 8 and of each pair of chunks the 32 columns x / 8: one scale
+// block.  Eight lanes that store together write the same columns of eight tokens, which the swizzle spreads over all banks.
 __device__ __forceinline__ unsigned clean(unsigned w, unsigned top, unsigned& bad) {   // a pair of 16-bit floats with NaN and infinities taken out
   if ((w & top) == top) { w &= 0xffff0000u; bad = 1; }
   if ((w & (top << 16)) == (top << 16)) { w &= 0x0000ffffu; bad = 1; }
@@ -177,17 +184,13 @@ __device__ __forceinline__ unsigned clean(unsigned w, unsigned top, unsigned& ba
 }
 // 16-byte unit u (8 columns) of a token's row in a chunk, swizzled
 __device__ __forceinline__ int unit_at(int token, int u) { return token * 128 + ((u ^ (token & 7)) << 4); }
-__device__ __forceinline__ uint4 fetch(const unsigned char* p) {
-  const V8 v = ld_stream(p);
-  return make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
-}
 __device__ __forceinline__ void copy16(unsigned char* dst, const unsigned char* src, bool live) {   // zeros where there is no row
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(su(dst)), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_left() { asm volatile("cp.async.wait_group %0;" :: "n"(LEFT) : "memory"); }
 
-// The token tiles of a CTA one after another, through its segments.
+// The pages of a CTA one after another, through its segments.
 struct Cursor {
   Segment s;
   unsigned n;
@@ -197,22 +200,18 @@ struct Cursor {
   __device__ __forceinline__ void step(Control& k) {
     if (live() && ++t == s.t1) { s = segment(k, ++n, true); t = s.t0; }
   }
-  // page of tokens first .. of the tile, -1 where there is none, and how many of the page's tokens there are
-  __device__ __forceinline__ int page(int first, int& tokens) const {
-    const int at = t * kTile + (first & 64);               // tokens: at most 2^26
-    tokens = live() ? max(0, min(64, s.tokens - at)) : 0;
-    return tokens ? __ldg(s.table + (at >> 6)) : -1;
-  }
+  // the page of its half h (0, 1) of the tile, and how many of its tokens there are
+  __device__ __forceinline__ int page(int h) const { return live() && (2 * t + h) * kPageTokens < s.tokens ? __ldg(s.table + 2 * t + h) : -1; }
+  __device__ __forceinline__ int tokens(int h) const { return live() ? max(0, min(kPageTokens, s.tokens - (2 * t + h) * kPageTokens)) : 0; }   // tokens: at most 2^26
   // steps of a sequence do not see all of its last S - 1 tokens: a value that is not finite must not reach the others through 0 * NaN
   __device__ __forceinline__ bool careful(const AttnArgs& a) const { return live() && s.b >= 0 && a.S > 1 && (t + 1) * kTile > s.tokens - (a.S - 1); }
 };
 
-__device__ __forceinline__ void store16(unsigned at, unsigned x, unsigned y, unsigned z, unsigned w) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-// 2^-d as a pair of f16 (255 stands for NaN), and four E4M3 codes times it: exact but for what falls below f16's 2^-24.
-__device__ __forceinline__ unsigned f16_scale(unsigned d) {
-  const unsigned h = d <= 14 ? (15u - d) << 10 : d == 255 ? 0x7e00u : 1024u >> min(d - 14u, 31u);
+// 2^(byte - most) as a pair of f16 (byte 255: NaN), and four E4M3 codes times it: exact but for what falls below f16's 2^-24.
+__device__ __forceinline__ unsigned f16_scale(unsigned most, unsigned byte) {
+  const int d = max((int)(most - byte), 0);
+  unsigned h = d <= 14 ? (15u - d) << 10 : 1024u >> min(d - 14, 31);
+  if (byte == 255) h = 0x7e00u;
   return h * 0x10001u;
 }
 __device__ __forceinline__ void mx8_to_f16x4(unsigned codes, unsigned scale, unsigned& lo, unsigned& hi) {
@@ -220,170 +219,166 @@ __device__ __forceinline__ void mx8_to_f16x4(unsigned codes, unsigned scale, uns
       : "=r"(lo), "=r"(hi) : "r"(codes), "r"(scale));
 }
 
-// What the warp has just written of one or two chunks, without its NaN and infinities (rare: a rolled loop, out of the way).
-__device__ __noinline__ void clean_pair(unsigned char* chunk, int steps, int token, int l, unsigned top, unsigned& bad) {
-  __syncwarp();                                              // units are cleaned by the lane that owns their column here, whoever wrote them
+// What the lane has just written of chunk units, without its NaN and infinities (rare: a rolled loop, out of the way).
+__device__ __forceinline__ void clean_units(unsigned char* chunk, int token, int unit, int units, unsigned top, unsigned& bad) {
 #pragma unroll 1
-  for (int x = 0; x < steps; ++x) {
-    uint4* at = reinterpret_cast<uint4*>(chunk + (x >> 1) * kChunk + unit_at(token + 4 * (x & 1), l));
-    unsigned b = 0;
+  for (int x = unit; x < unit + units; ++x) {
+    uint4* at = reinterpret_cast<uint4*>(chunk + unit_at(token, x));
     const uint4 v = *at;
-    *at = make_uint4(clean(v.x, top, b), clean(v.y, top, b), clean(v.z, top, b), clean(v.w, top, b));
-    bad |= b << (x & 1);
+    *at = make_uint4(clean(v.x, top, bad), clean(v.y, top, bad), clean(v.z, top, bad), clean(v.w, top, bad));
   }
 }
 
 // Chunks are handed over in pairs (0 1, 2 3, 4 5, 6 7, and the rope chunk), a fence and an arrival for each; a pair's slots are free as soon as
-// its 128 columns of P V are done, the rope slot before that.  The page of a tile is looked up two tiles ahead.  Its codes are fetched into registers,
-// all in one go, when the tile before it has been handed over: they arrive while that one is multiplied.  (Fetched pair by pair
-// they wait for each other: a warp has few scoreboards to wait on.)  bf16 rows are twice as many registers: pairs 0 and 1 are held, the others are
-// copied straight into their slots once those are free.
+// its 128 columns of P V are done, the rope slot before that.  The page of a tile is looked up two tiles ahead; its codes are fetched into registers in one
+// go when the tile before it has been handed over, and arrive during its products (with two tiles under way a warp would wait for
+// both: it has few scoreboards).
 template <bool MX8>
-__device__ void load_tiles(const AttnArgs& a, Control& k, unsigned char* slots, int tid) {
-  const int lane = tid & 31, first = (tid >> 5) * 8, sub = lane >> 3, l = lane & 7;
-  const int row0 = (first & 56) + sub;                       // row in its page of step 0's token
+struct Loader {
+  const AttnArgs& a;
+  Control& k;
+  unsigned char* slots;
+  int tid, lane, token, block;
   Cursor cur;
-  cur.start(k);
-  constexpr int kHeld = MX8 ? 4 : 2, kPer = MX8 ? 2 : 4;     // held[pair][step]: 16 codes; bf16 held[pair][chunk, step]: 8 columns
-  uint4 held[kHeld][kPer], scales = make_uint4(0u, 0u, 0u, 0u);   // lane x holds the scale bytes of token `first` + x % 8
-#pragma unroll
-  for (int p = 0; p < kHeld; ++p)
-#pragma unroll
-    for (int x = 0; x < kPer; ++x) held[p][x] = scales;
-  // where the thread's first unit of step j goes (j even, j odd): the swizzle of token 8 w + 4 j + sub is sub + 4 j
-  unsigned put[2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int unit = MX8 ? 2 * (l & 3) + (l >> 2) : l;
-    put[x] = su(slots) + (MX8 ? (l >> 2) * kChunk : 0) + (first + sub) * 128 + ((unit ^ (sub + 4 * x)) << 4);
+  int next_id;
+  // a tile on its way: MXFP8, 32 codes of each pair of chunks, the token's scale bytes; bf16, 32 columns of two pairs
+  V16 code[4];
+  V8 scales;
+  const unsigned char* page;
+  int tokens;                                                // of the page (none of one that the cache does not hold)
+  bool careful;
+  __device__ __forceinline__ Loader(const AttnArgs& a, Control& k, unsigned char* slots, int t) : a(a), k(k), slots(slots), tid(t), lane(t & 31),
+      token((t >> 5) * 8 + (t & 7)), block(lane >> 3) {
+    cur.start(k);
+    next_id = cur.page(tid >> 8);
   }
-  int tokens = 0, next_tokens;                               // tokens of this warp's page in this tile (none of a page that the cache does not hold)
-  const unsigned char* page = a.cache;
-  int next_id = cur.page(first, next_tokens);
-  bool careful = false, next_careful = cur.careful(a);
-  for (unsigned i = 0;; ++i) {                               // i: tiles done by this CTA
-    if (!cur.live()) return;
-    tokens = next_id >= 0 && next_id < a.pages ? next_tokens : 0;
-    careful = next_careful;
-    if (tokens > 0) {
-      page = a.cache + next_id * a.page_stride;
-      if (MX8) scales = fetch(page + kPageScales + ((first & 56) + (lane & 7)) * (kLatent / 32));
-      else scales = make_uint4(0u, 0u, 0u, 0u);
+  // the tile at the cursor, whose page was looked up before; false at the end
+  __device__ __forceinline__ bool fetch() {
+    if (!cur.live()) return false;
+    tokens = next_id >= 0 && next_id < a.pages ? cur.tokens(tid >> 8) : 0;
+    careful = cur.careful(a);
+    page = a.cache + (tokens ? next_id : 0) * a.page_stride;
+    const int row = token & 63;
+    if (tokens) {                                            // rows behind the last token are in the page: read, and not used
+      if (MX8) {
+        scales = ld_stream(page + kPageScales + row * (kLatent / 32));
 #pragma unroll
-      for (int p = 0; p < kHeld; ++p)
+        for (int p = 0; p < 4; ++p) code[p] = ld_stream32(page + row * kLatent + p * 128 + block * 32);
+      } else {
 #pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-          const int row = row0 + 4 * (x & 1);
-          held[p][x] = fetch(MX8 ? page + row * kLatent + p * 128 + l * 16 : page + (row * kRow + (2 * p + (x >> 1)) * 64 + l * 8) * 2);
+        for (int x = 0; x < 4; ++x) {                        // bf16 pages are 16-byte aligned
+          const unsigned char* src = page + (row * kRow + (x >> 1) * 128 + block * 32 + (x & 1) * 16) * 2;
+          const V8 lo = ld_stream(src), hi = ld_stream(src + 16);
+          code[x] = V16{{lo.w[0], lo.w[1], lo.w[2], lo.w[3], hi.w[0], hi.w[1], hi.w[2], hi.w[3]}};
         }
+      }
+    } else {
+      code[0] = code[1] = code[2] = code[3] = V16{{0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u}};
+      scales = V8{{0u, 0u, 0u, 0u}};
     }
     cur.step(k);
-    next_id = cur.page(first, next_tokens);
-    next_careful = cur.careful(a);
-    auto copy = [&](int c) {
+    next_id = cur.page(tid >> 8);
+    return true;
+  }
+  __device__ __forceinline__ void hand_over(int p) {
+    fence_async();
+    __syncwarp();
+    if (lane == 0) arrive(k.full[p]);
+  }
+  __device__ __forceinline__ void copy(int c) {              // a chunk straight into its slot: eight threads to a token
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int row = row0 + 4 * j;
-        const unsigned char* src = MX8 ? page + kPageRope + row * 128 + l * 16 : page + (row * kRow + c * 64 + l * 8) * 2;
-        copy16(slots + c * kChunk + unit_at(first + 4 * j + sub, l), row < tokens ? src : reinterpret_cast<const unsigned char*>(a.q), row < tokens);
-      }
-    };
-    const bool whole = tokens == kPageTokens;
-    int E = 0;
-    if (MX8) {
-      // E, the largest exponent of the warp's tokens, and each block's distance from it (255: a scale that is NaN)
-      const uint4 nan = make_uint4(__vcmpeq4(scales.x, ~0u), __vcmpeq4(scales.y, ~0u), __vcmpeq4(scales.z, ~0u), __vcmpeq4(scales.w, ~0u));
-      unsigned m = __vmaxu4(__vmaxu4(scales.x & ~nan.x, scales.y & ~nan.y), __vmaxu4(scales.z & ~nan.z, scales.w & ~nan.w));
-      m = max(max(m & 255u, (m >> 8) & 255u), max((m >> 16) & 255u, m >> 24));
-      m = (first & 56) + (lane & 7) < tokens ? m : 0u;
-      m = __reduce_max_sync(0xffffffffu, m);
-      m = min(max(m, (unsigned)(127 + kLeastE)), (unsigned)(127 + kMostE));
-      E = (int)m - 127;
-      m *= 0x01010101u;
-      scales = make_uint4(__vsubus4(m, scales.x) | nan.x, __vsubus4(m, scales.y) | nan.y, __vsubus4(m, scales.z) | nan.z, __vsubus4(m, scales.w) | nan.w);
+    for (int x = 0; x < 2; ++x) {
+      const int at = (tid >> 8) * 64 + ((tid >> 3) & 31) + 32 * x, row = at & 63, unit = tid & 7;
+      const bool there = row < tokens;
+      const unsigned char* src = MX8 ? page + kPageRope + row * 128 + unit * 16 : page + (row * kRow + c * 64 + unit * 8) * 2;
+      copy16(slots + c * kChunk + unit_at(at, unit), there ? src : reinterpret_cast<const unsigned char*>(a.q), there);
     }
-    unsigned bad = 0;                                        // bit j: step j's token has a value that is not finite
+  }
+  __device__ __forceinline__ void clean_copy(int c, unsigned i) {
 #pragma unroll 1
-    for (int p = 0; p < 4; ++p) {                            // rolled: the pair at hand is always held[0]; unrolled, the warps wait for instructions
+    for (int x = 0; x < 2; ++x) {
+      const int at = (tid >> 8) * 64 + ((tid >> 3) & 31) + 32 * x;
+      unsigned bad = 0;
+      clean_units(slots + c * kChunk, at, tid & 7, 1, 0x7f80u, bad);
+      if (bad) atomicOr(&k.poison[i & 1][at >> 5], 1u << (at & 31));
+    }
+  }
+  // tile i of the CTA into the slots
+  __device__ __forceinline__ void put(unsigned i) {
+    const bool there = (token & 63) < tokens;
+    unsigned bad = 0, most = 0;                              // bad: the token has a value that is not finite
+    if (MX8) {
+      // the largest scale byte of the warp's tokens but for 255 (NaN): four lanes share a token, each looks at four of its sixteen bytes, counted up by one
+      // modulo 256
+      const unsigned w = block < 2 ? (block == 0 ? scales.w[0] : scales.w[1]) : (block == 2 ? scales.w[2] : scales.w[3]);
+      unsigned m;
+      asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(((w & 0x00ff00ffu) + 0x00010001u) & 0x00ff00ffu), "r"((((w >> 8) & 0x00ff00ffu) + 0x00010001u) & 0x00ff00ffu));
+      m = max(m & 0xffffu, m >> 16);
+      most = __reduce_max_sync(0xffffffffu, there ? m : 0u);
+      most = min(max(most, (unsigned)(128 + kLeastE)), (unsigned)(128 + kMostE)) - 1;
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      uint4 u[4];
+      if (MX8) {                                             // converted before the wait
+        const unsigned s = f16_scale(most, (scales.w[p] >> (block * 8)) & 0xffu);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          mx8_to_f16x4(code[p].w[2 * x], s, u[x].x, u[x].y);
+          mx8_to_f16x4(code[p].w[2 * x + 1], s, u[x].z, u[x].w);
+        }
+      } else if (p < 2) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const V16& v = code[2 * p + (x >> 1)];
+          u[x] = make_uint4(v.w[4 * (x & 1)], v.w[4 * (x & 1) + 1], v.w[4 * (x & 1) + 2], v.w[4 * (x & 1) + 3]);
+        }
+      }
       if (i > 0) wait(k, k.empty[p], (i - 1) & 1);
       if (p == 0) {
         if (tid < 4) k.poison[(i + 1) & 1][tid] = 0;         // the tile before this one has been read, the next is not there yet
-        if (MX8 && lane == 0) k.exponent[i & 1][first >> 3] = E;
+        if (MX8 && lane == 0) k.exponent[token >> 3] = (int)most - 127;   // E
+        if ((tid & 255) == 0) k.tokens[tid >> 8] = tokens;
         copy(8);
         copies_commit();
       }
-      const unsigned at = 2 * p * kChunk;
-      if (MX8) {
-        unsigned sc[2];
-        uint4 u[2], v[2];
+      if (MX8 || p < 2) {
+        unsigned char* chunk = slots + (2 * p + (block >> 1)) * kChunk;
+        if (tokens < kPageTokens && !there) u[0] = u[1] = u[2] = u[3] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) sc[j] = __shfl_sync(0xffffffffu, scales.x, 4 * j + sub);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {                        // 16 codes: two units of one chunk
-          const unsigned s = f16_scale((sc[j] >> ((l >> 1) * 8)) & 0xffu);
-          // lanes 0..3 and 4..7 write to the same columns of two chunks: in opposite order, so that no bank is wanted twice
-          const uint4 q = held[0][j];
-          const bool back = l >= 4;
-          mx8_to_f16x4(back ? q.z : q.x, s, u[j].x, u[j].y); mx8_to_f16x4(back ? q.w : q.y, s, u[j].z, u[j].w);
-          mx8_to_f16x4(back ? q.x : q.z, s, v[j].x, v[j].y); mx8_to_f16x4(back ? q.y : q.w, s, v[j].z, v[j].w);
-        }
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            if (row0 + 4 * j >= tokens) u[j] = v[j] = make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          store16(put[j & 1] + at + j * 512, u[j].x, u[j].y, u[j].z, u[j].w);
-          store16((put[j & 1] + at + j * 512) ^ 16u, v[j].x, v[j].y, v[j].z, v[j].w);
-        }
-#pragma unroll
-        for (int x = 0; x + 1 < kHeld; ++x)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) held[x][j] = held[x + 1][j];
-        scales.x = scales.y; scales.y = scales.z; scales.z = scales.w;
-      } else if (p < kHeld) {
-#pragma unroll
-        for (int x = 0; x < kPer; ++x) {
-          uint4 u = held[0][x];
-          if (!whole && row0 + 4 * (x & 1) >= tokens) u = make_uint4(0u, 0u, 0u, 0u);
-          store16(put[x & 1] + at + (x >> 1) * kChunk + (x & 1) * 512, u.x, u.y, u.z, u.w);
-          held[0][x] = held[1][x];
-        }
-      } else if (p == 2) {
+        for (int x = 0; x < 4; ++x) *reinterpret_cast<uint4*>(chunk + unit_at(token, (block & 1) * 4 + x)) = u[x];
+        if (careful) clean_units(chunk, token, (block & 1) * 4, 4, MX8 ? 0x7c00u : 0x7f80u, bad);
+      } else if (p == 2) {                                   // the other half of bf16 pages: copied
         copy(4); copy(5);
         copies_commit();
         if (i > 0) wait(k, k.empty[3], (i - 1) & 1);
         copy(6); copy(7);
         copies_commit();
         copies_left<1>();
+        if (careful) { clean_copy(4, i); clean_copy(5, i); }
       } else {
         copies_left<0>();
+        if (careful) { clean_copy(6, i); clean_copy(7, i); }
       }
-      if (careful) clean_pair(slots + 2 * p * kChunk, 4, first + sub, l, MX8 ? 0x7c00u : 0x7f80u, bad);
-      fence_async();
-      __syncwarp();
-      if (lane == 0) arrive(k.full[p]);
+      hand_over(p);
     }
     copies_left<0>();
     if (careful) {
-      clean_pair(slots + 8 * kChunk, 2, first + sub, l, 0x7f80u, bad);
-      for (int j = 0; j < 2; ++j) {
-        const int token = first + 4 * j + sub;
-        if ((bad >> j) & 1u) atomicOr(&k.poison[i & 1][token >> 5], 1u << (token & 31));
-      }
+      clean_copy(8, i);
+      if (bad) atomicOr(&k.poison[i & 1][token >> 5], 1u << (token & 31));
     }
-    fence_async();
-    __syncwarp();
-    if (lane == 0) arrive(k.full[4]);
+    hand_over(4);
   }
-}
+  __device__ __forceinline__ void run() {
+    for (unsigned i = 0; fetch(); ++i) put(i);
+  }
+};
 
 // ---- MMA ------------------------------------------------------------------------------------------------------------------------------
 template <bool MX8>
 __device__ void issue_tiles(Control& k, unsigned q, unsigned p, unsigned slots) {
-  const unsigned tmem = *(volatile unsigned*)&k.tmem, o = tmem, sc = tmem + kTmemS, sr = tmem + (MX8 ? kTmemR : kTmemS), tq = tmem + kTmemQ;
-  unsigned dq = operand(q, 16), dk = operand(slots, 16), dp = operand(p, 16), dv = operand(slots, kChunk);
+  const unsigned tmem = *(volatile unsigned*)&k.tmem, sc = tmem + kTmemS, sr = tmem + (MX8 ? kTmemR : kTmemS);
+  const unsigned dq = operand(q, 16), dk = operand(slots, 16), dp = operand(p, 16), dv = operand(slots, kChunk);
   unsigned lead;
   asm volatile("{.reg .pred e; elect.sync _|e, 0xffffffff; selp.u32 %0, 1, 0, e;}" : "=r"(lead));
   unsigned i = 0;
@@ -398,20 +393,23 @@ __device__ void issue_tiles(Control& k, unsigned q, unsigned p, unsigned slots) 
         fence_after();
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          mma_ws(lead, sc, dq + ((2 * c * kQChunk + (j >> 2) * kQChunk + (j & 3) * 32) >> 4), dk + ((2 * c * kChunk + (j >> 2) * kChunk + (j & 3) * 32) >> 4),
+          mma_ws(lead, sc, dq + (((2 * c + (j >> 2)) * kQChunk + (j & 3) * 32) >> 4), dk + (((2 * c + (j >> 2)) * kChunk + (j & 3) * 32) >> 4),
                  shape_of(!MX8, 0), c + j > 0);
       }
       wait(k, k.full[4], i & 1);
       fence_after();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mma_ws_tmem(lead, sr, tq + j * 8, dk + ((8 * kChunk + j * 32) >> 4), shape_of(true, 0), !MX8 || j > 0);
+      for (int j = 0; j < 4; ++j) mma_ws_tmem(lead, sr, tmem + kTmemQ + j * 8, dk + ((8 * kChunk + j * 32) >> 4), shape_of(true, 0), !MX8 || j > 0);
       commit(lead, k.s_full);
+      wait(k, k.p_full, i & 1);
+      if (t == s.t0 && n > 0) wait(k, k.o_free, (n - 1) & 1);
+      fence_after();
 #pragma unroll 1
       for (int u = 0; u < 4; ++u) {                          // 128 output columns each
-        if (u == 0) { wait(k, k.p_full[0], i & 1); wait(k, k.p_full[1], i & 1); fence_after(); }
 #pragma unroll
         for (int x = 0; x < 8; ++x)                          // 16 tokens each
-          mma_ws(lead, o + u * 64, dp + (((x >> 2) * kQChunk + (x & 3) * 32) >> 4), dv + ((u * 2 * kChunk + x * 2048) >> 4), shape_of(!MX8, 1), t > s.t0 || x > 0);
+          mma_ws(lead, tmem + u * 64, dp + (((x >> 2) * kQChunk + (x & 3) * 32) >> 4), dv + ((u * 2 * kChunk + x * 2048) >> 4), shape_of(!MX8, 1),
+                 t > s.t0 || x > 0);
         commit(lead, k.empty[u]);
       }
     }
@@ -451,7 +449,7 @@ __device__ __forceinline__ void fetch_q_rope(const AttnArgs& a, const Segment& s
 }
 // They have come: for MXFP8 pages made f16 where they lie, the row's largest element brought to 2^14 .. 2^15, each thread what it fetched.
 template <bool MX8>
-__device__ __forceinline__ void q_ready(Control& k, unsigned char* q, int tid) {
+__device__ __forceinline__ void q_ready(Control& k, unsigned char* q, unsigned n, int tid) {
   copies_left<0>();
   if (MX8) {
     const int r = tid >> 2;
@@ -467,7 +465,7 @@ __device__ __forceinline__ void q_ready(Control& k, unsigned char* q, int tid) {
     const int e = (int)(top >> 7);                           // exponent field of the largest element; 0: a row of zeros (or of subnormals), 255: not finite
     const int shift = e == 0 || e == 255 ? 0 : e - 127 - 14; // q' = q * 2^-shift
     const float up = __uint_as_float((unsigned)(127 - shift) << 23);
-    if ((tid & 3) == 0) k.row_scale[r] = __uint_as_float((unsigned)(127 + shift) << 23);
+    if ((tid & 3) == 0) k.row_scale[n & 1][r] = __uint_as_float((unsigned)(127 + shift) << 23);
 #pragma unroll 4
     for (int i = 0; i < 16; ++i) {
       const int unit = 4 * i + (tid & 3);
@@ -489,48 +487,54 @@ __device__ __forceinline__ void softmax_barrier(int rows) {
   if (rows == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
   else asm volatile("bar.sync 2, 128;" ::: "memory");
 }
+__device__ __forceinline__ bool softmax_vote(int rows, bool mine) {   // the same barrier, and whether it is true for one of them
+  unsigned any;
+  if (rows == 0) asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, 1, 128, p; selp.u32 %0, 1, 0, q;}" : "=r"(any) : "r"((unsigned)mine) : "memory");
+  else asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, 2, 128, p; selp.u32 %0, 1, 0, q;}" : "=r"(any) : "r"((unsigned)mine) : "memory");
+  return any != 0;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 
-// Warp w: rows 32 (w % 2) .. of the tile, page w / 2 % 2 of each token tile, its tokens 32 (w / 4) ..; of O the columns on the same lanes, two accumulators of
-// the four.
+// Warp w: rows 32 (w % 2) .. of the tile, of page w / 2 % 2 of each token tile 32 tokens (32 (w / 4) ..), of O the columns on the same lanes of two
+// accumulators.
 template <bool MX8>
 __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned char* q, unsigned char* p_mem, int tid) {
-  const int r = tid & 63, half = (tid >> 6) & 1, part = tid >> 7, rows32 = (tid >> 5) & 1;
+  const int r = tid & 63, half = (tid >> 6) & 1, part = tid >> 7, rows32 = (tid >> 5) & 1, first = half * 64 + part * 32;
   const unsigned lanes = (unsigned)((tid >> 5) & 3) << 21;   // this warp's 32 lanes of tensor memory
   const unsigned tmem = *(volatile unsigned*)&k.tmem + lanes, o = tmem + part * 128, sc = tmem + kTmemS + part * 32, tq = tmem + kTmemQ;
-  unsigned char* p_row = p_mem + half * kQChunk;
-  Segment s = segment(k, 0, false);
-  if (s.t1 == 0) return;
-  fetch_q(a, s, q, tid);
-  if (part == 0) fetch_q_rope(a, s, tq, r);
-  q_ready<MX8>(k, q, tid);
+  {
+    const Segment s = segment(k, 0, false);
+    if (s.t1 == 0) return;
+    fetch_q(a, s, q, tid);
+    if (part == 0) fetch_q_rope(a, s, tq, r);
+    q_ready<MX8>(k, q, 0, tid);
+  }
   unsigned i = 0;
   for (unsigned n = 0;; ++n) {
-    s = segment(k, n, true);
+    const Segment s = segment(k, n, true);
     if (s.t1 == 0) return;
     int seen = s.tokens;                                     // tokens that the row sees
     if (s.b >= 0) seen = s.tokens - (a.S - 1 - min((s.row0 + r) / a.heads, a.S - 1));
-    float row_scale = 1.f, m = -INFINITY, l = 0.f;                            // the maximum that P and O are relative to, and this thread's share of the sum
+    float row_scale = 1.f;
+    float m = -INFINITY, l = 0.f;                            // the maximum that P and O are relative to, and this thread's share of the sum
+#pragma unroll 1
     for (int t = s.t0; t < s.t1; ++t, ++i) {
-      const int base = t * kTile + half * 64;
-      int live = min(32, max(0, seen - base - part * 32));   // visible ones of this thread's 32 tokens
-      if (live > 0) {
-        const int id = __ldg(s.table + (base >> 6));
-        if (id < 0 || id >= a.pages) live = 0;
-      }
       wait(k, k.s_full, i & 1);
       fence_after();
+      if (MX8 && t == s.t0) row_scale = *(volatile float*)&k.row_scale[n & 1][r];
       unsigned raw[32];
       tmem_ld32(sc, raw);
       int ex[4] = {0, 0, 0, 0};                              // E of the thread's four runs of 8 tokens
+      // visible ones of this thread's 32 tokens, if not below 0 or above 32
+      const int live = min(seen - t * kTile - half * 64, *(volatile int*)&k.tokens[half]) - part * 32;
       if (MX8) {
         unsigned rope[32];
         tmem_ld32(sc + (kTmemR - kTmemS), rope);
-        if (t == s.t0) row_scale = *(volatile float*)&k.row_scale[r];
+        const int4 e = *reinterpret_cast<const int4*>(&k.exponent[first >> 3]);
+        ex[0] = e.x; ex[1] = e.y; ex[2] = e.z; ex[3] = e.w;
         tmem_wait_ld();
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          ex[g] = *(volatile int*)&k.exponent[i & 1][half * 8 + part * 4 + g];
           const f32x2 f = f2_splat(row_scale * __uint_as_float((unsigned)(ex[g] + 127) << 23));
 #pragma unroll
           for (int j = 8 * g; j < 8 * g + 8; j += 2) {
@@ -542,50 +546,43 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned char* q, u
       } else {
         tmem_wait_ld();
       }
-      // the maximum of the visible scores, and a sum that turns NaN where one is not finite
       if (a.flip) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) raw[j] ^= 0x80000000u;
       }
-      const bool whole = __all_sync(0xffffffffu, live == 32);
-      if (!whole) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) raw[j] = j < live ? raw[j] : 0u;
-      }
-      f32x2 odd2[2] = {f2_splat(0.f), f2_splat(0.f)};
-#pragma unroll
-      for (int j = 0; j < 16; ++j) odd2[j & 1] = f2_fma(f2_pack(__uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1])), f2_splat(0.f), odd2[j & 1]);
-      if (!whole) {
+      if (live < 32) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) raw[j] = j < live ? raw[j] : 0xff800000u;
       }
+      if (s.b >= 0 && a.S > 1 && live > 0) {                 // the bad values of tokens that not all rows see were taken out
+        if (*(volatile unsigned*)&k.poison[i & 1][2 * half + part] & (~0u >> (32 - min(live, 32)))) l = NAN;
+      }
+      // the row's maximum only where a score is above what P and O are relative to: all four threads of all 32 rows vote
       float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < 16; ++j) tops[j >> 2] = max3(tops[j >> 2], __uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1]));
-      float odd, odd1, top = fmaxf(fmaxf(fmaf(tops[0], a.c, (float)ex[0]), fmaf(tops[1], a.c, (float)ex[1])), fmaxf(fmaf(tops[2], a.c, (float)ex[2]), fmaf(tops[3], a.c, (float)ex[3])));
-      f2_unpack(f2_add(odd2[0], odd2[1]), odd, odd1);
-      odd += odd1;
-      const unsigned mine = *(volatile unsigned*)&k.poison[i & 1][2 * half + part];
-      if (mine && live > 0 && (mine & (~0u >> (32 - live)))) odd = NAN;
-      l += odd;
-      k.best[2 * part + half][r] = top;
-      softmax_barrier(rows32);
-      top = fmaxf(fmaxf(k.best[0][r], k.best[1][r]), fmaxf(k.best[2][r], k.best[3][r]));
-      if (t == s.t0) m = top;
-      else if (__any_sync(0xffffffffu, top > m + kLag)) {    // O of these 32 rows catches up with the maximum
-        const float best = fmaxf(m, top), f = best == -INFINITY ? 1.f : exp2_fast(m - best);
-        l *= f;
-        m = best;
+      float top = fmaxf(fmaxf(fmaf(tops[0], a.c, (float)ex[0]), fmaf(tops[1], a.c, (float)ex[1])), fmaxf(fmaf(tops[2], a.c, (float)ex[2]), fmaf(tops[3], a.c, (float)ex[3])));
+      if (softmax_vote(rows32, t == s.t0 || top > m + kLag)) {
+        k.best[2 * part + half][r] = top;
+        softmax_barrier(rows32);
+        top = fmaxf(fmaxf(k.best[0][r], k.best[1][r]), fmaxf(k.best[2][r], k.best[3][r]));
+        if (t == s.t0) {
+          m = top;
+        } else {                                             // O of these 32 rows catches up with the maximum; the product before this one is done
+          const float best = fmaxf(m, top), f = best == -INFINITY ? 1.f : exp2_fast(m - best);
+          l *= f;
+          m = best;
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          unsigned v[32];
-          tmem_ld32(o + c, v);
-          tmem_wait_ld();
+          for (int c = 0; c < 128; c += 32) {
+            unsigned v[32];
+            tmem_ld32(o + c, v);
+            tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
-          tmem_st32(o + c, v);
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
+            tmem_st32(o + c, v);
+          }
+          tmem_wait_st();
         }
-        tmem_wait_st();
       }
       const float off = kTop - (m == -INFINITY ? 0.f : m);
 #pragma unroll
@@ -607,20 +604,21 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned char* q, u
             pw[j] = pack_bf2(e0, e1);
           }
         }
-        *reinterpret_cast<uint4*>(p_row + unit_at(r, part * 4 + g)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
+        *reinterpret_cast<uint4*>(p_mem + half * kQChunk + unit_at(r, part * 4 + g)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
         float s0, s1;
         f2_unpack(f2_add(sum2[0], sum2[1]), s0, s1);
         l = fmaf(s0 + s1, __uint_as_float((unsigned)(127 - ex[g]) << 23), l);   // a token's weight itself, without its 2^E
       }
       fence_async();
       fence_before();
-      arrive(k.p_full[part]);
+      arrive(k.p_full);
     }
     // the last product with this segment's queries is done: the next segment's take their place while P V goes on
     const Segment next = segment(k, n + 1, false);
     if (next.t1 > 0) {
       fetch_q(a, next, q, tid);
       if (part == 0) fetch_q_rope(a, next, tq, r);
+      q_ready<MX8>(k, q, n + 1, tid);
     }
     // this stretch's unnormalised outputs, maximum and sum
     wait(k, k.empty[3], (i - 1) & 1);
@@ -630,6 +628,7 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned char* q, u
     k.best[2 * part + half][r] = l;
     softmax_barrier(rows32);
     if (half + part == 0 && live_row) a.sums[at * kRows + r] = make_float2(m, (k.best[0][r] + k.best[1][r]) + (k.best[2][r] + k.best[3][r]));
+    softmax_barrier(rows32);                                 // the sums are read before a maximum takes their place
     float* dst = a.parts + at * kPartFloats + r * kLatent + part * 256 + half * 64;
 #pragma unroll 1
     for (int c = 0; c < 128; c += 32) {
@@ -637,13 +636,13 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned char* q, u
       tmem_ld32(o + c, v);
       tmem_wait_ld();
       if (live_row) {
-        float* d = dst + (c >> 6) * 128 + (c & 63);
 #pragma unroll
         for (int j = 0; j < 32; j += 8)
-          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(d + j), K3G_I8(v, j) : "memory");
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(dst + (c >> 6) * 128 + (c & 63) + j), K3G_I8(v, j) : "memory");
       }
     }
-    if (next.t1 > 0) q_ready<MX8>(k, q, tid);                // the next segment's first product overwrites O: after these loads
+    fence_before();
+    arrive(k.o_free);
   }
 }
 
@@ -677,7 +676,7 @@ __device__ void plan(const AttnArgs& a, Control& k, int ptok, int lane) {
       }
       s.t1 = 0;
     }
-    if (n >= kRing) wait(k, k.ring_empty[n % kRing], (n / kRing - 1) & 1);
+    if (n >= kRing) wait(k, k.ring_empty[n % kRing], (n / kRing - 1) & 1, 1000);
     if (lane == 0) {
       k.ring[n % kRing] = s;
       arrive(k.ring_full[n % kRing]);
@@ -710,12 +709,13 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
   if (lane == 31) k.scan[warp] = upto;
   if (tid == 0) {
     auto init = [](unsigned long long& bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(su(&bar)), "r"(n)); };
+    for (int u = 0; u < 5; ++u) init(k.full[u], kLoaders / 32);
 #pragma unroll 1
-    for (int c = 0; c < 5; ++c) init(k.full[c], kLoaders / 32);
+    for (int u = 0; u < 4; ++u) init(k.empty[u], 1);
+    init(k.s_full, 1); init(k.p_full, kSoftmax);
 #pragma unroll 1
-    for (int u = 0; u < 4; ++u) { init(k.empty[u], 1); init(k.ring_full[u], 1); init(k.ring_empty[u], kReaders); }
-    init(k.p_full[0], kSoftmax / 2); init(k.p_full[1], kSoftmax / 2);
-    init(k.q_full, kSoftmax); init(k.s_full, 1);
+    for (int u = 0; u < kRing; ++u) { init(k.ring_full[u], 1); init(k.ring_empty[u], kReaders); }
+    init(k.q_full, kSoftmax); init(k.o_free, kSoftmax);
     k.abort = 0;
 #pragma unroll 1
     for (int i = 0; i < 8; ++i) k.poison[i >> 2][i & 3] = 0;
@@ -755,15 +755,15 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
   if (busy) {
     unsigned char *q = smem, *p = q + kSmemQ, *slots = p + kSmemP;
     if (warp < kSoftmax / 32) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
       softmax_tiles<MX8>(a, k, q, p, tid);
     } else if (warp < (kSoftmax + kLoaders) / 32) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-      load_tiles<MX8>(a, k, slots, tid - kSoftmax);
+      Loader<MX8>(a, k, slots, tid - kSoftmax).run();
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
       if (warp == (kSoftmax + kLoaders) / 32) issue_tiles<MX8>(k, su(q), su(p), su(slots));
-      else if (warp == (kSoftmax + kLoaders) / 32 + 1) plan(a, k, ptok, lane);
+      else if (warp == (kSoftmax + kLoaders) / 32 + 3) plan(a, k, ptok, lane);
     }
   }
   fence_before();
@@ -892,7 +892,8 @@ K3G_API int k3g_latent_attn(const void* q, long long q_stride, const void* cache
   if (prefix_pages > 0) { K3G_REQUIRE_PTR(prefix_table); K3G_REQUIRE_PTR(prefix_len); }
   if (max_pages > 0) K3G_REQUIRE_PTR(block_table);
   const long long unit = cache_mx8 ? 1 : 2, page = cache_mx8 ? kMx8Page : 2 * kBf16Page;
-  K3G_REQUIRE(q_stride % 8 == 0 && layer_off * unit % 16 == 0 && page_stride * unit % 16 == 0, K3G_EALIGN);
+  const long long grain = cache_mx8 ? 32 : 16;
+  K3G_REQUIRE(q_stride % 8 == 0 && layer_off * unit % grain == 0 && page_stride * unit % grain == 0 && (reinterpret_cast<uintptr_t>(cache) & (grain - 1)) == 0, K3G_EALIGN);
   K3G_REQUIRE(S > 0 && heads > 0 && q_stride >= (long long)heads * kRow && layer_off >= 0 && page_stride * unit >= layer_off * unit + page, K3G_ESHAPE);
   K3G_REQUIRE(B <= kMaxBatch && (long long)S * heads <= kMaxRowsPerSeq && prefix_pages <= (1 << 20) && max_pages <= (1 << 20), K3G_ELIMIT);
   const Space sp = space_of(B, S, heads);

@@ -78,7 +78,7 @@ K3G_API int k3g_latent_mx8_store(const void* rows, long long row_stride, const v
                                  long long page_stride, long long pages, int T, void* stream) {
   K3G_REQUIRE_PTR(rows); K3G_REQUIRE_PTR(slot_mapping); K3G_REQUIRE_PTR(cache);
   K3G_REQUIRE_ALIGNED(rows); K3G_REQUIRE_ALIGNED(cache);
-  K3G_REQUIRE(row_stride % 8 == 0 && layer_off % 16 == 0 && page_stride % 16 == 0, K3G_EALIGN);
+  K3G_REQUIRE(row_stride % 8 == 0 && layer_off % 32 == 0 && page_stride % 32 == 0 && (reinterpret_cast<uintptr_t>(cache) & 31u) == 0, K3G_EALIGN);
   K3G_REQUIRE(T >= 0 && pages >= 0 && pages < (1ll << 31), K3G_ESHAPE);
   if (T == 0) return K3G_OK;
   K3G_REQUIRE(row_stride >= kRow && layer_off >= 0 && page_stride >= layer_off + kMx8Page, K3G_ESHAPE);
@@ -91,7 +91,7 @@ K3G_API int k3g_latent_mx8_gather(const void* cache, const void* block_table, lo
                                   const void* lens, void* out, int n, void* stream) {
   K3G_REQUIRE_PTR(cache); K3G_REQUIRE_PTR(block_table); K3G_REQUIRE_PTR(lens); K3G_REQUIRE_PTR(out);
   K3G_REQUIRE_ALIGNED(cache); K3G_REQUIRE_ALIGNED(out);
-  K3G_REQUIRE(layer_off % 16 == 0 && page_stride % 16 == 0, K3G_EALIGN);
+  K3G_REQUIRE(layer_off % 32 == 0 && page_stride % 32 == 0 && (reinterpret_cast<uintptr_t>(cache) & 31u) == 0, K3G_EALIGN);
   K3G_REQUIRE(n >= 0 && pages >= 0 && pages < (1ll << 31), K3G_ESHAPE);
   if (n == 0) return K3G_OK;
   K3G_REQUIRE(layer_off >= 0 && page_stride >= layer_off + kMx8Page, K3G_ESHAPE);

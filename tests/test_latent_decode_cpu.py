@@ -26,15 +26,15 @@ VERIFY = dict(target=P, target_stride=100, draft=P, draft_stride=100, ids=P, u=P
 @pytest.mark.parametrize("name,base,change,code", [
     ("k3g_latent_mx8_store", STORE, dict(rows=None), -1), ("k3g_latent_mx8_store", STORE, dict(slots=None), -1),
     ("k3g_latent_mx8_store", STORE, dict(rows=P + 8), -3), ("k3g_latent_mx8_store", STORE, dict(row_stride=580), -3),
-    ("k3g_latent_mx8_store", STORE, dict(row_stride=568), -2), ("k3g_latent_mx8_store", STORE, dict(layer_off=8), -3),
-    ("k3g_latent_mx8_store", STORE, dict(page_stride=MX8_PAGE + 8), -3), ("k3g_latent_mx8_store", STORE, dict(page_stride=MX8_PAGE - 16), -2),
-    ("k3g_latent_mx8_store", STORE, dict(layer_off=16), -2), ("k3g_latent_mx8_store", STORE, dict(layer_off=-16), -2),
+    ("k3g_latent_mx8_store", STORE, dict(row_stride=568), -2), ("k3g_latent_mx8_store", STORE, dict(layer_off=16), -3), ("k3g_latent_mx8_store", STORE, dict(cache=P + 16), -3),
+    ("k3g_latent_mx8_store", STORE, dict(page_stride=MX8_PAGE + 8), -3), ("k3g_latent_mx8_store", STORE, dict(page_stride=MX8_PAGE - 32), -2),
+    ("k3g_latent_mx8_store", STORE, dict(layer_off=32), -2), ("k3g_latent_mx8_store", STORE, dict(layer_off=-32), -2),
     ("k3g_latent_mx8_store", STORE, dict(T=-1), -2), ("k3g_latent_mx8_store", STORE, dict(pages=-1), -2), ("k3g_latent_mx8_store", STORE, dict(T=0), 0),
     ("k3g_latent_mx8_gather", GATHER, dict(lens=None), -1), ("k3g_latent_mx8_gather", GATHER, dict(out=P + 4), -3),
-    ("k3g_latent_mx8_gather", GATHER, dict(page_stride=16), -2), ("k3g_latent_mx8_gather", GATHER, dict(n=-1), -2), ("k3g_latent_mx8_gather", GATHER, dict(n=0), 0),
+    ("k3g_latent_mx8_gather", GATHER, dict(page_stride=32), -2), ("k3g_latent_mx8_gather", GATHER, dict(cache=P + 16), -3), ("k3g_latent_mx8_gather", GATHER, dict(n=-1), -2), ("k3g_latent_mx8_gather", GATHER, dict(n=0), 0),
     ("k3g_latent_attn", ATTN, dict(q=None), -1), ("k3g_latent_attn", ATTN, dict(lens=None), -1), ("k3g_latent_attn", ATTN, dict(prefix_table=None), -1),
     ("k3g_latent_attn", ATTN, dict(prefix_len=None), -1), ("k3g_latent_attn", ATTN, dict(table=None), -1), ("k3g_latent_attn", ATTN, dict(workspace=None), -1),
-    ("k3g_latent_attn", ATTN, dict(q=P + 2), -3), ("k3g_latent_attn", ATTN, dict(q_stride=24 * ROW + 4), -3), ("k3g_latent_attn", ATTN, dict(workspace=P + 8), -3),
+    ("k3g_latent_attn", ATTN, dict(q=P + 2), -3), ("k3g_latent_attn", ATTN, dict(cache=P + 16), -3), ("k3g_latent_attn", ATTN, dict(q_stride=24 * ROW + 4), -3), ("k3g_latent_attn", ATTN, dict(workspace=P + 8), -3),
     ("k3g_latent_attn", ATTN, dict(mx8=0, page_stride=PAGE * ROW + 4), -3), ("k3g_latent_attn", ATTN, dict(mx8=0, page_stride=PAGE * ROW - 8), -2),
     ("k3g_latent_attn", ATTN, dict(q_stride=23 * ROW), -2), ("k3g_latent_attn", ATTN, dict(S=0), -2), ("k3g_latent_attn", ATTN, dict(heads=0), -2),
     ("k3g_latent_attn", ATTN, dict(B=-1), -2), ("k3g_latent_attn", ATTN, dict(max_pages=-1), -2), ("k3g_latent_attn", ATTN, dict(B=4097), -5),

@@ -389,7 +389,7 @@ int k3g_latent_gather(const void* slab, const void* block_table, long long page_
 
 /* ---- decoding with drafts over the latent cache (no counterpart in the reference, which only prefills) ---------- */
 /* The cache is paged as k3g_mla_prep writes it: pages of 64 tokens, a page table per sequence, `layer_off` the layer's place in
- * a page.  bf16 pages are 64 rows of 576 (512 latent columns, 64 rope columns); offsets and strides in elements.  MXFP8 pages
+ * a page.  bf16 pages are 64 rows of 576 (512 latent columns, 64 rope columns); offsets and strides in elements (multiples of 16 here).  MXFP8 pages
  * are 41984 bytes in three planes -- 64 x 512 E4M3 codes, 64 x 64 bf16 (the rope columns as they are), 64 x 16 UE8M0 scale bytes --
  * 656 bytes a token instead of 1152; offsets and strides in bytes, multiples of 32, and the cache 32-byte aligned.  `pages` is the number of pages the cache
  * holds: a table entry outside [0, pages) is never read, and neither is one behind the last token of its sequence. */

@@ -13,8 +13,8 @@
 // a captured graph follows them.  Nothing is accumulated by atomics: the same inputs give the same bits.
 //
 // One CTA per SM, warps with fixed roles, one token tile after another:
-//   1 planning warp  this CTA's stretches, one after another, into a ring that the others read;
-//   16 loader warps  fetch the next tile into registers and make 16-bit floats of it in 128-byte-swizzled shared memory, nine 16 KB chunks of 64
+//   1 planning warp  this CTA's stretches, one after another, and the pages of their tiles, into rings that the others read;
+//   8 loader warps   fetch the next tile into registers and make 16-bit floats of it in 128-byte-swizzled shared memory, nine 16 KB chunks of 64
 //                    columns;
 //   1 MMA warp       S = Q K^T (64 x 128, two chunks at a time as they come) and O += P V (64 x 512 in tensor memory), both tcgen05.mma.ws, M = 64;
 //   8 softmax warps  S from tensor memory, running maximum, P = 2^(S - m) rounded to 16 bits into shared memory; O scaled, read and written out.
@@ -26,7 +26,7 @@
 //
 // Types.  bf16 pages are multiplied as bf16.  MXFP8 codes become f16, not bf16: one conversion and one product for two codes, a third of what bf16
 // takes (which has no conversion from E4M3), and the loaders' instructions are what a tile waits for.  f16 has the bits (a code has four), but not the
-// range, so exponents are taken out: of the scales of 8 tokens the largest, E (K' = code * 2^(e - E), exact down to 2^-24 of 2^E), of
+// range, so exponents are taken out: of the scales of 16 tokens the largest, E (K' = code * 2^(e - E), exact down to 2^-24 of 2^E), of
 // a query row its own (the largest element is brought to 2^14..2^15; what that costs is below 2^-39 of it).  They come back in f32: S = 2^(E + row) S' + S_rope
 // (the rope columns are multiplied as bf16 into a second accumulator), and P' = 2^(S + E - m), with m the running maximum of S + E, so
 // that P' V' has the weight of P V.  P is rounded because both operands of the matrix instructions are 16 bits; the sums of P stay unrounded in f32.
@@ -43,16 +43,16 @@ namespace {
 
 constexpr int kMaxBatch = 4096, kMaxRowsPerSeq = 1 << 15, kMaxCtas = 160;
 constexpr int kRows = 64, kTile = 2 * kPageTokens;           // query rows and tokens of a tile
-constexpr int kSoftmax = 256, kLoaders = 512, kThreads = kSoftmax + kLoaders + 128;   // the last four warps: MMAs, planning, two idle
+constexpr int kSoftmax = 256, kLoaders = 256, kThreads = kSoftmax + kLoaders + 128;   // the last four warps: MMAs, planning, two idle
 constexpr int kChunk = kTile * 128, kQChunk = kRows * 128;   // 64 columns of a tile's tokens, of its rows, at 16 bits
 constexpr int kSmemQ = 8 * kQChunk, kSmemP = 2 * kQChunk, kSmemK = 9 * kChunk, kSmem = kSmemQ + kSmemP + kSmemK + 1024;
 // tensor memory columns: O 0..255 (four accumulators of 128 output columns, 64 on either half of the lanes), S 256..319 (a page on either
 // half), the rope columns' part of S 320..383 (MXFP8), the queries' rope columns 384..415 (the same on both halves)
 constexpr int kTmemS = 256, kTmemR = 320, kTmemQ = 384;
-constexpr int kLeastE = -80, kMostE = 120;                   // exponents of 8 tokens: sums of 2^-E stay in range
+constexpr int kLeastE = -80, kMostE = 120;                   // exponents of 16 tokens: sums of 2^-E stay in range
 constexpr float kLag = 4.f, kTop = 10.f;
 constexpr int kPartFloats = kRows * kLatent;                 // a part's outputs; its 64 (maximum, sum) pairs lie in a table of their own
-constexpr int kWaitLimit = 1 << 20, kRing = 4, kReaders = (kSoftmax + kLoaders) / 32 + 1;
+constexpr int kWaitLimit = 1 << 20, kRing = 4, kReaders = kSoftmax / 32 + 1, kTiles = 4;
 constexpr int kStart = 2;
 
 struct AttnArgs {
@@ -87,22 +87,26 @@ struct Segment {                     // one CTA's stretch of one row tile
   int row0;                          // first row: of all rows (prefix) or of the sequence's rows
   int t0, t1;                        // token tiles (none: the end)
   int tokens;                        // tokens of the prefix / of the sequence
-  const int* table;
+};
+struct Tile {                        // where a tile's pages are
+  const unsigned char* page[2];
+  int tokens[2];                     // of each (none of a page that the cache does not hold)
+  int live, careful;                 // 0: the end; steps of a sequence do not all see all of its tokens
 };
 
 // ---- barriers and tensor memory -----------------------------------------------------------------------------------------------
 struct Control {
-  unsigned long long full[5], empty[4], s_full, p_full, q_full, o_free;
-  unsigned long long ring_full[kRing], ring_empty[kRing];
+  unsigned long long full[5], empty[4], s_full, s_read, p_full, q_full, o_free;
+  unsigned long long ring_full[kRing], ring_empty[kRing], tile_full[kTiles], tile_empty[kTiles];
+  Tile tile[kTiles];
   Segment ring[kRing];
   unsigned tmem;
   int abort;
   int first_tile, first_at;
   long long left;
   unsigned poison[2][4];                                      // tokens of a tile with values that are not finite (tiles by turns)
-  alignas(16) int exponent[16];
-  int tokens[2];                                // of a tile: E of each 8 tokens, and how many there are in either page
-  float row_scale[2][kRows];                                  // 2^(what was taken out of a query row), segments by turns
+  int exponent[8], tokens[2];                                // of a tile: E of each 16 tokens, and how many there are in either page
+  signed char row_shift[2][kRows];                            // the power of two that was taken out of a query row, segments by turns
   union {
     float best[4][kRows];                                     // the maxima of a page, and at a segment's end the sums
     long long scan[kThreads / 32];                            // before the first
@@ -175,7 +179,7 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // ---- loaders ----------------------------------------------------------------------------------------------------------------------
-// Warp w looks after tokens 8 w .. + 7 of a tile, lane x after token 8 w + x % 8 and of each pair of chunks the 32 columns x / 8: one scale
+// Warp w looks after tokens 16 w .. + 15 of a tile, lane x after tokens 16 w + x % 8 and + 8 and of each pair of chunks the 32 columns x / 8: one scale
 // block.  Eight lanes that store together write the same columns of eight tokens, which the swizzle spreads over all banks.
 __device__ __forceinline__ unsigned clean(unsigned w, unsigned top, unsigned& bad) {   // a pair of 16-bit floats with NaN and infinities taken out
   if ((w & top) == top) { w &= 0xffff0000u; bad = 1; }
@@ -184,35 +188,26 @@ __device__ __forceinline__ unsigned clean(unsigned w, unsigned top, unsigned& ba
 }
 // 16-byte unit u (8 columns) of a token's row in a chunk, swizzled
 __device__ __forceinline__ int unit_at(int token, int u) { return token * 128 + ((u ^ (token & 7)) << 4); }
-__device__ __forceinline__ void copy16(unsigned char* dst, const unsigned char* src, bool live) {   // zeros where there is no row
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(su(dst)), "l"(src), "r"(live ? 16 : 0) : "memory");
+// Shared memory is addressed by 32-bit numbers here: the compiler does not see the address space behind the aligned base pointer.
+__device__ __forceinline__ void copy16(unsigned dst, const unsigned char* src, bool live) {   // zeros where there is no row
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void store16(unsigned at, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 load16(unsigned at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_left() { asm volatile("cp.async.wait_group %0;" :: "n"(LEFT) : "memory"); }
 
-// The pages of a CTA one after another, through its segments.
-struct Cursor {
-  Segment s;
-  unsigned n;
-  int t;
-  __device__ __forceinline__ void start(Control& k) { n = 0; s = segment(k, 0, true); t = s.t0; }
-  __device__ __forceinline__ bool live() const { return s.t1 > 0; }
-  __device__ __forceinline__ void step(Control& k) {
-    if (live() && ++t == s.t1) { s = segment(k, ++n, true); t = s.t0; }
-  }
-  // the page of its half h (0, 1) of the tile, and how many of its tokens there are
-  __device__ __forceinline__ int page(int h) const { return live() && (2 * t + h) * kPageTokens < s.tokens ? __ldg(s.table + 2 * t + h) : -1; }
-  __device__ __forceinline__ int tokens(int h) const { return live() ? max(0, min(kPageTokens, s.tokens - (2 * t + h) * kPageTokens)) : 0; }   // tokens: at most 2^26
-  // steps of a sequence do not see all of its last S - 1 tokens: a value that is not finite must not reach the others through 0 * NaN
-  __device__ __forceinline__ bool careful(const AttnArgs& a) const { return live() && s.b >= 0 && a.S > 1 && (t + 1) * kTile > s.tokens - (a.S - 1); }
-};
-
 // 2^(byte - most) as a pair of f16 (byte 255: NaN), and four E4M3 codes times it: exact but for what falls below f16's 2^-24.
 __device__ __forceinline__ unsigned f16_scale(unsigned most, unsigned byte) {
-  const int d = max((int)(most - byte), 0);
-  unsigned h = d <= 14 ? (15u - d) << 10 : 1024u >> min(d - 14, 31);
-  if (byte == 255) h = 0x7e00u;
-  return h * 0x10001u;
+  const float f = __uint_as_float((unsigned)max((int)(byte + 127 - most), 0) << 23);
+  const __half2 h = __floats2half2_rn(f, f);
+  return byte == 255 ? 0x7e007e00u : *reinterpret_cast<const unsigned*>(&h);
 }
 __device__ __forceinline__ void mx8_to_f16x4(unsigned codes, unsigned scale, unsigned& lo, unsigned& hi) {
   asm("{.reg .b16 a, b; .reg .b32 x, y; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 x, a; cvt.rn.f16x2.e4m3x2 y, b; mul.rn.f16x2 %0, x, %3; mul.rn.f16x2 %1, y, %3;}"
@@ -220,157 +215,205 @@ __device__ __forceinline__ void mx8_to_f16x4(unsigned codes, unsigned scale, uns
 }
 
 // What the lane has just written of chunk units, without its NaN and infinities (rare: a rolled loop, out of the way).
-__device__ __forceinline__ void clean_units(unsigned char* chunk, int token, int unit, int units, unsigned top, unsigned& bad) {
+__device__ __forceinline__ void clean_units(unsigned chunk, int token, int unit, int units, unsigned top, unsigned& bad) {
 #pragma unroll 1
   for (int x = unit; x < unit + units; ++x) {
-    uint4* at = reinterpret_cast<uint4*>(chunk + unit_at(token, x));
-    const uint4 v = *at;
-    *at = make_uint4(clean(v.x, top, bad), clean(v.y, top, bad), clean(v.z, top, bad), clean(v.w, top, bad));
+    const unsigned at = chunk + unit_at(token, x);
+    const uint4 v = load16(at);
+    store16(at, make_uint4(clean(v.x, top, bad), clean(v.y, top, bad), clean(v.z, top, bad), clean(v.w, top, bad)));
   }
 }
 
 // Chunks are handed over in pairs (0 1, 2 3, 4 5, 6 7, and the rope chunk), a fence and an arrival for each; a pair's slots are free as soon as
-// its 128 columns of P V are done, the rope slot before that.  The page of a tile is looked up two tiles ahead; its codes are fetched into registers in one
-// go when the tile before it has been handed over, and arrive during its products (with two tiles under way a warp would wait for
-// both: it has few scoreboards).
+// its 128 columns of P V are done, the rope slot before that.  The next tile's codes are fetched into registers when this one has been
+// handed over (any earlier and a warp, which has few scoreboards, would wait for new data with the old), in portions: what a tile's loads
+// move (80 KB, 64 bytes a clock) would else be in the way of the softmax warps' reads of S and stores of P.
 template <bool MX8>
 struct Loader {
   const AttnArgs& a;
   Control& k;
-  unsigned char* slots;
+  unsigned slots, put_at[4];                                 // the thread's units of its first token's first pair of chunks; the other token's are 1024 bytes on
   int tid, lane, token, block;
-  Cursor cur;
-  int next_id;
-  // a tile on its way: MXFP8, 32 codes of each pair of chunks, the token's scale bytes; bf16, 32 columns of two pairs
-  V16 code[4];
-  V8 scales;
-  const unsigned char* page;
-  int tokens;                                                // of the page (none of one that the cache does not hold)
-  bool careful;
-  __device__ __forceinline__ Loader(const AttnArgs& a, Control& k, unsigned char* slots, int t) : a(a), k(k), slots(slots), tid(t), lane(t & 31),
-      token((t >> 5) * 8 + (t & 7)), block(lane >> 3) {
-    cur.start(k);
-    next_id = cur.page(tid >> 8);
+  // a tile on its way: MXFP8, 32 codes of each pair of chunks, the scale bytes; bf16, 32 columns of two pairs; of two tokens each
+  V16 code[4][2];
+  V8 scales[2];
+  struct Where {
+    const unsigned char* page;
+    int tokens;
+    bool careful, live;
+  } here, next;
+  __device__ __forceinline__ Loader(const AttnArgs& a, Control& k, unsigned slots, int t) : a(a), k(k), slots(slots), tid(t), lane(t & 31),
+      token((t >> 5) * 16 + (t & 7)), block(lane >> 3) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) put_at[x] = slots + (block >> 1) * kChunk + unit_at(token, (block & 1) * 4 + x);
   }
-  // the tile at the cursor, whose page was looked up before; false at the end
-  __device__ __forceinline__ bool fetch() {
-    if (!cur.live()) return false;
-    tokens = next_id >= 0 && next_id < a.pages ? cur.tokens(tid >> 8) : 0;
-    careful = cur.careful(a);
-    page = a.cache + (tokens ? next_id : 0) * a.page_stride;
-    const int row = token & 63;
-    if (tokens) {                                            // rows behind the last token are in the page: read, and not used
-      if (MX8) {
-        scales = ld_stream(page + kPageScales + row * (kLatent / 32));
-#pragma unroll
-        for (int p = 0; p < 4; ++p) code[p] = ld_stream32(page + row * kLatent + p * 128 + block * 32);
-      } else {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {                        // bf16 pages are 16-byte aligned
-          const unsigned char* src = page + (row * kRow + (x >> 1) * 128 + block * 32 + (x & 1) * 16) * 2;
-          const V8 lo = ld_stream(src), hi = ld_stream(src + 16);
-          code[x] = V16{{lo.w[0], lo.w[1], lo.w[2], lo.w[3], hi.w[0], hi.w[1], hi.w[2], hi.w[3]}};
-        }
+  __device__ __forceinline__ Where where(unsigned i) {       // tile i's pages
+    wait(k, k.tile_full[i % kTiles], (i / kTiles) & 1);
+    const Tile& t = k.tile[i % kTiles];
+    const int half = tid >> 7;
+    Where w;
+    w.page = *(const unsigned char* const volatile*)&t.page[half];
+    w.tokens = *(const volatile int*)&t.tokens[half];
+    w.live = *(const volatile int*)&t.live != 0;
+    w.careful = *(const volatile int*)&t.careful != 0;
+    __syncwarp();
+    if (lane == 0) arrive(k.tile_empty[i % kTiles]);
+    return w;
+  }
+  template <int P0, int P1>
+  __device__ __forceinline__ void load(const Where& w) {     // code[P0 .. P1)
+    if (w.tokens) {                                          // rows behind the last token are in the page: read, and not used
+      const unsigned char* src = w.page + (token & 63) * (MX8 ? kLatent : 2 * kRow) + block * (MX8 ? 32 : 64);
+      if (MX8 && P0 == 0) {
+        const unsigned char* sc = w.page + kPageScales + (token & 63) * (kLatent / 32);
+        scales[0] = ld_stream(sc);
+        scales[1] = ld_stream(sc + 8 * (kLatent / 32));
       }
+#pragma unroll
+      for (int p = P0; p < P1; ++p)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) code[p][g] = ld_stream32(src + (MX8 ? p * 128 + g * 8 * kLatent : (p >> 1) * 256 + (p & 1) * 32 + g * 16 * kRow));
     } else {
-      code[0] = code[1] = code[2] = code[3] = V16{{0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u}};
-      scales = V8{{0u, 0u, 0u, 0u}};
+      if (P0 == 0) scales[0] = scales[1] = V8{{0u, 0u, 0u, 0u}};
+#pragma unroll
+      for (int p = P0; p < P1; ++p) code[p][0] = code[p][1] = V16{{0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u}};
     }
-    cur.step(k);
-    next_id = cur.page(tid >> 8);
-    return true;
   }
   __device__ __forceinline__ void hand_over(int p) {
     fence_async();
     __syncwarp();
     if (lane == 0) arrive(k.full[p]);
   }
-  __device__ __forceinline__ void copy(int c) {              // a chunk straight into its slot: eight threads to a token
+  __device__ __forceinline__ void copy(int c) {              // a chunk of the warp's tokens straight into its slot: eight lanes to a token
+    const int at = (tid >> 5) * 16 + (lane >> 3), unit = lane & 7;
+    const unsigned char* src = MX8 ? here.page + kPageRope + (at & 63) * 128 + unit * 16 : here.page + ((at & 63) * kRow + c * 64 + unit * 8) * 2;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int at = (tid >> 8) * 64 + ((tid >> 3) & 31) + 32 * x, row = at & 63, unit = tid & 7;
-      const bool there = row < tokens;
-      const unsigned char* src = MX8 ? page + kPageRope + row * 128 + unit * 16 : page + (row * kRow + c * 64 + unit * 8) * 2;
-      copy16(slots + c * kChunk + unit_at(at, unit), there ? src : reinterpret_cast<const unsigned char*>(a.q), there);
+    for (int x = 0; x < 4; ++x) {
+      const bool there = (at & 63) + 4 * x < here.tokens;
+      copy16(slots + c * kChunk + unit_at(at + 4 * x, unit), there ? src + x * (MX8 ? 4 * 128 : 8 * kRow) : reinterpret_cast<const unsigned char*>(a.q), there);
     }
   }
   __device__ __forceinline__ void clean_copy(int c, unsigned i) {
 #pragma unroll 1
-    for (int x = 0; x < 2; ++x) {
-      const int at = (tid >> 8) * 64 + ((tid >> 3) & 31) + 32 * x;
+    for (int x = 0; x < 4; ++x) {
+      const int at = (tid >> 5) * 16 + (lane >> 3) + 4 * x;
       unsigned bad = 0;
-      clean_units(slots + c * kChunk, at, tid & 7, 1, 0x7f80u, bad);
+      clean_units(slots + c * kChunk, at, lane & 7, 1, 0x7f80u, bad);
       if (bad) atomicOr(&k.poison[i & 1][at >> 5], 1u << (at & 31));
     }
   }
-  // tile i of the CTA into the slots
-  __device__ __forceinline__ void put(unsigned i) {
-    const bool there = (token & 63) < tokens;
-    unsigned bad = 0, most = 0;                              // bad: the token has a value that is not finite
+  struct Units { uint4 u[2][4]; };
+  __device__ __forceinline__ Units convert(int p, unsigned most) {   // of pair p (bf16: 0 or 1)
+    Units o;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      if (MX8) {
+        const unsigned s = f16_scale(most, (scales[g].w[p] >> (block * 8)) & 0xffu);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          mx8_to_f16x4(code[p][g].w[2 * x], s, o.u[g][x].x, o.u[g][x].y);
+          mx8_to_f16x4(code[p][g].w[2 * x + 1], s, o.u[g][x].z, o.u[g][x].w);
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const V16& v = code[(2 * p + (x >> 1)) & 3][g];
+          o.u[g][x] = make_uint4(v.w[4 * (x & 1)], v.w[4 * (x & 1) + 1], v.w[4 * (x & 1) + 2], v.w[4 * (x & 1) + 3]);
+        }
+      }
+    }
+    if (here.tokens < kPageTokens) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if ((token & 63) + 8 * g >= here.tokens) o.u[g][0] = o.u[g][1] = o.u[g][2] = o.u[g][3] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    return o;
+  }
+  unsigned bad[2];                                           // the thread's tokens have values that are not finite
+  __device__ __forceinline__ void put(int p, const Units& o) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) store16(put_at[x] + 2 * p * kChunk + g * 1024, o.u[g][x]);
+    if (here.careful) {
+      clean_units(slots + (2 * p + (block >> 1)) * kChunk, token, (block & 1) * 4, 4, MX8 ? 0x7c00u : 0x7f80u, bad[0]);
+      clean_units(slots + (2 * p + (block >> 1)) * kChunk, token + 8, (block & 1) * 4, 4, MX8 ? 0x7c00u : 0x7f80u, bad[1]);
+    }
+  }
+  __device__ __forceinline__ void empty(unsigned i, int p) { if (i > 0) wait(k, k.empty[p], (i - 1) & 1); }
+  // tile i of the CTA into the slots, and the next one on its way
+  __device__ __forceinline__ void tile(unsigned i) {
+    unsigned most = 0;
+    bad[0] = bad[1] = 0;
     if (MX8) {
       // the largest scale byte of the warp's tokens but for 255 (NaN): four lanes share a token, each looks at four of its sixteen bytes, counted up by one
       // modulo 256
-      const unsigned w = block < 2 ? (block == 0 ? scales.w[0] : scales.w[1]) : (block == 2 ? scales.w[2] : scales.w[3]);
-      unsigned m;
-      asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(((w & 0x00ff00ffu) + 0x00010001u) & 0x00ff00ffu), "r"((((w >> 8) & 0x00ff00ffu) + 0x00010001u) & 0x00ff00ffu));
-      m = max(m & 0xffffu, m >> 16);
-      most = __reduce_max_sync(0xffffffffu, there ? m : 0u);
-      most = min(max(most, (unsigned)(128 + kLeastE)), (unsigned)(128 + kMostE)) - 1;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const unsigned w = block < 2 ? (block == 0 ? scales[g].w[0] : scales[g].w[1]) : (block == 2 ? scales[g].w[2] : scales[g].w[3]);
+        unsigned m;
+        asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(((w & 0x00ff00ffu) + 0x00010001u) & 0x00ff00ffu), "r"((((w >> 8) & 0x00ff00ffu) + 0x00010001u) & 0x00ff00ffu));
+        if ((token & 63) + 8 * g < here.tokens) most = max(most, max(m & 0xffffu, m >> 16));
+      }
+      most = min(max(__reduce_max_sync(0xffffffffu, most), (unsigned)(128 + kLeastE)), (unsigned)(128 + kMostE)) - 1;
     }
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      uint4 u[4];
-      if (MX8) {                                             // converted before the wait
-        const unsigned s = f16_scale(most, (scales.w[p] >> (block * 8)) & 0xffu);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          mx8_to_f16x4(code[p].w[2 * x], s, u[x].x, u[x].y);
-          mx8_to_f16x4(code[p].w[2 * x + 1], s, u[x].z, u[x].w);
-        }
-      } else if (p < 2) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const V16& v = code[2 * p + (x >> 1)];
-          u[x] = make_uint4(v.w[4 * (x & 1)], v.w[4 * (x & 1) + 1], v.w[4 * (x & 1) + 2], v.w[4 * (x & 1) + 3]);
-        }
-      }
-      if (i > 0) wait(k, k.empty[p], (i - 1) & 1);
-      if (p == 0) {
-        if (tid < 4) k.poison[(i + 1) & 1][tid] = 0;         // the tile before this one has been read, the next is not there yet
-        if (MX8 && lane == 0) k.exponent[token >> 3] = (int)most - 127;   // E
-        if ((tid & 255) == 0) k.tokens[tid >> 8] = tokens;
-        copy(8);
-        copies_commit();
-      }
-      if (MX8 || p < 2) {
-        unsigned char* chunk = slots + (2 * p + (block >> 1)) * kChunk;
-        if (tokens < kPageTokens && !there) u[0] = u[1] = u[2] = u[3] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) *reinterpret_cast<uint4*>(chunk + unit_at(token, (block & 1) * 4 + x)) = u[x];
-        if (careful) clean_units(chunk, token, (block & 1) * 4, 4, MX8 ? 0x7c00u : 0x7f80u, bad);
-      } else if (p == 2) {                                   // the other half of bf16 pages: copied
-        copy(4); copy(5);
-        copies_commit();
-        if (i > 0) wait(k, k.empty[3], (i - 1) & 1);
-        copy(6); copy(7);
-        copies_commit();
-        copies_left<1>();
-        if (careful) { clean_copy(4, i); clean_copy(5, i); }
-      } else {
-        copies_left<0>();
-        if (careful) { clean_copy(6, i); clean_copy(7, i); }
-      }
-      hand_over(p);
+    const Units u0 = convert(0, most);
+    empty(i, 0);
+    if (tid < 4) k.poison[(i + 1) & 1][tid] = 0;             // the tile before this one has been read, the next is not there yet
+    if (MX8 && lane == 0) k.exponent[tid >> 5] = (int)most - 127;   // E
+    if ((tid & 127) == 0) k.tokens[tid >> 7] = here.tokens;
+    put(0, u0);
+    hand_over(0);
+    copy(8);
+    copies_commit();
+    const Units u1 = convert(1, most);
+    empty(i, 1);
+    put(1, u1);
+    hand_over(1);
+    if (MX8) {
+      const Units u2 = convert(2, most);
+      empty(i, 2);
+      put(2, u2);
+      hand_over(2);
+      const Units u3 = convert(3, most);
+      empty(i, 3);
+      put(3, u3);
+      hand_over(3);
+      next = where(i + 1);
+    } else {                                                 // the other half of bf16 pages is copied
+      next = where(i + 1);
+      load<0, 4>(next);
+      empty(i, 2);
+      copy(4); copy(5);
+      copies_commit();
+      empty(i, 3);
+      copy(6); copy(7);
+      copies_commit();
+      copies_left<1>();
+      if (here.careful) { clean_copy(4, i); clean_copy(5, i); }
+      hand_over(2);
+      copies_left<0>();
+      if (here.careful) { clean_copy(6, i); clean_copy(7, i); }
+      hand_over(3);
     }
     copies_left<0>();
-    if (careful) {
+    if (here.careful) {
       clean_copy(8, i);
-      if (bad) atomicOr(&k.poison[i & 1][token >> 5], 1u << (token & 31));
+      if (bad[0]) atomicOr(&k.poison[i & 1][token >> 5], 1u << (token & 31));
+      if (bad[1]) atomicOr(&k.poison[i & 1][token >> 5], 256u << (token & 31));
     }
     hand_over(4);
+    if (MX8) {
+      load<0, 3>(next);
+      wait(k, k.s_read, i & 1);
+      load<3, 4>(next);
+    }
+    here = next;
   }
   __device__ __forceinline__ void run() {
-    for (unsigned i = 0; fetch(); ++i) put(i);
+    here = where(0);
+    load<0, 4>(here);
+    for (unsigned i = 0; here.live; ++i) tile(i);
   }
 };
 
@@ -425,7 +468,7 @@ __device__ __forceinline__ const __nv_bfloat16* query(const AttnArgs& a, const S
   return a.q + ((s.b < 0 ? 0 : s.b * a.S) + step) * a.q_stride + (at - step * a.heads) * kRow;
 }
 // The latent columns of a segment's queries on their way into shared memory, four threads to a row; zeros where the tile has no row.
-__device__ __forceinline__ void fetch_q(const AttnArgs& a, const Segment& s, unsigned char* q, int tid) {
+__device__ __forceinline__ void fetch_q(const AttnArgs& a, const Segment& s, unsigned q, int tid) {
   const int r = tid >> 2;
   const unsigned char* src = reinterpret_cast<const unsigned char*>(query(a, s, r));
 #pragma unroll 4
@@ -449,7 +492,7 @@ __device__ __forceinline__ void fetch_q_rope(const AttnArgs& a, const Segment& s
 }
 // They have come: for MXFP8 pages made f16 where they lie, the row's largest element brought to 2^14 .. 2^15, each thread what it fetched.
 template <bool MX8>
-__device__ __forceinline__ void q_ready(Control& k, unsigned char* q, unsigned n, int tid) {
+__device__ __forceinline__ void q_ready(Control& k, unsigned q, unsigned n, int tid) {
   copies_left<0>();
   if (MX8) {
     const int r = tid >> 2;
@@ -457,25 +500,25 @@ __device__ __forceinline__ void q_ready(Control& k, unsigned char* q, unsigned n
 #pragma unroll 4
     for (int i = 0; i < 16; ++i) {
       const int unit = 4 * i + (tid & 3);
-      const uint4 x = *reinterpret_cast<const uint4*>(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7));
+      const uint4 x = load16(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7));
       top = max(top, absmax8(V8{{x.x, x.y, x.z, x.w}}));
     }
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e = (int)(top >> 7);                           // exponent field of the largest element; 0: a row of zeros (or of subnormals), 255: not finite
-    const int shift = e == 0 || e == 255 ? 0 : e - 127 - 14; // q' = q * 2^-shift
+    const int shift = e == 0 || e == 255 ? 0 : max(e - 127 - 14, -120);   // q' = q * 2^-shift
     const float up = __uint_as_float((unsigned)(127 - shift) << 23);
-    if ((tid & 3) == 0) k.row_scale[n & 1][r] = __uint_as_float((unsigned)(127 + shift) << 23);
+    if ((tid & 3) == 0) k.row_shift[n & 1][r] = (signed char)shift;
 #pragma unroll 4
     for (int i = 0; i < 16; ++i) {
       const int unit = 4 * i + (tid & 3);
-      uint4* at = reinterpret_cast<uint4*>(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7));
-      const uint4 x = *at;
+      const unsigned at = q + (unit >> 3) * kQChunk + unit_at(r, unit & 7);
+      const uint4 x = load16(at);
       auto half = [&](unsigned w) {
         const __half2 h = __floats2half2_rn(bf_lo(w) * up, bf_hi(w) * up);
         return *reinterpret_cast<const unsigned*>(&h);
       };
-      *at = make_uint4(half(x.x), half(x.y), half(x.z), half(x.w));
+      store16(at, make_uint4(half(x.x), half(x.y), half(x.z), half(x.w)));
     }
   }
   fence_async();
@@ -498,7 +541,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) { float d; asm(
 // Warp w: rows 32 (w % 2) .. of the tile, of page w / 2 % 2 of each token tile 32 tokens (32 (w / 4) ..), of O the columns on the same lanes of two
 // accumulators.
 template <bool MX8>
-__device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned char* q, unsigned char* p_mem, int tid) {
+__device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigned p_mem, int tid) {
   const int r = tid & 63, half = (tid >> 6) & 1, part = tid >> 7, rows32 = (tid >> 5) & 1, first = half * 64 + part * 32;
   const unsigned lanes = (unsigned)((tid >> 5) & 3) << 21;   // this warp's 32 lanes of tensor memory
   const unsigned tmem = *(volatile unsigned*)&k.tmem + lanes, o = tmem + part * 128, sc = tmem + kTmemS + part * 32, tq = tmem + kTmemQ;
@@ -519,29 +562,30 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned char* q, u
     float m = -INFINITY, l = 0.f;                            // the maximum that P and O are relative to, and this thread's share of the sum
 #pragma unroll 1
     for (int t = s.t0; t < s.t1; ++t, ++i) {
-      wait(k, k.s_full, i & 1);
-      fence_after();
-      if (MX8 && t == s.t0) row_scale = *(volatile float*)&k.row_scale[n & 1][r];
-      unsigned raw[32];
-      tmem_ld32(sc, raw);
-      int ex[4] = {0, 0, 0, 0};                              // E of the thread's four runs of 8 tokens
+      // what the loaders left about the tile is read when they have handed it over: with S itself it would queue behind their next loads
+      wait(k, k.full[4], i & 1);
+      int ex[2] = {0, 0};                                    // E of the thread's two runs of 16 tokens
+      if (MX8) { ex[0] = *(volatile int*)&k.exponent[first >> 4]; ex[1] = *(volatile int*)&k.exponent[(first >> 4) + 1]; }
       // visible ones of this thread's 32 tokens, if not below 0 or above 32
       const int live = min(seen - t * kTile - half * 64, *(volatile int*)&k.tokens[half]) - part * 32;
+      unsigned mine = 0;                                     // those with values that are not finite, in tiles that not all rows see all of
+      if (s.b >= 0 && a.S > 1 && live > 0) mine = *(volatile unsigned*)&k.poison[i & 1][2 * half + part] & (~0u >> (32 - min(live, 32)));
+      wait(k, k.s_full, i & 1);
+      fence_after();
+      if (MX8 && t == s.t0) row_scale = __uint_as_float((unsigned)(127 + *(volatile signed char*)&k.row_shift[n & 1][r]) << 23);
+      unsigned raw[32];
+      tmem_ld32(sc, raw);
       if (MX8) {
         unsigned rope[32];
         tmem_ld32(sc + (kTmemR - kTmemS), rope);
-        const int4 e = *reinterpret_cast<const int4*>(&k.exponent[first >> 3]);
-        ex[0] = e.x; ex[1] = e.y; ex[2] = e.z; ex[3] = e.w;
+        const f32x2 f[2] = {f2_splat(row_scale * __uint_as_float((unsigned)(ex[0] + 127) << 23)), f2_splat(row_scale * __uint_as_float((unsigned)(ex[1] + 127) << 23))};
         tmem_wait_ld();
+        if ((tid & 31) == 0) arrive(k.s_read);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x2 f = f2_splat(row_scale * __uint_as_float((unsigned)(ex[g] + 127) << 23));
-#pragma unroll
-          for (int j = 8 * g; j < 8 * g + 8; j += 2) {
-            float u, v;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[j]), __uint_as_float(raw[j + 1])), f, f2_pack(__uint_as_float(rope[j]), __uint_as_float(rope[j + 1]))), u, v);
-            raw[j] = __float_as_uint(u); raw[j + 1] = __float_as_uint(v);
-          }
+        for (int j = 0; j < 32; j += 2) {
+          float u, v;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[j]), __uint_as_float(raw[j + 1])), f[j >> 4], f2_pack(__uint_as_float(rope[j]), __uint_as_float(rope[j + 1]))), u, v);
+          raw[j] = __float_as_uint(u); raw[j + 1] = __float_as_uint(v);
         }
       } else {
         tmem_wait_ld();
@@ -554,14 +598,12 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned char* q, u
 #pragma unroll
         for (int j = 0; j < 32; ++j) raw[j] = j < live ? raw[j] : 0xff800000u;
       }
-      if (s.b >= 0 && a.S > 1 && live > 0) {                 // the bad values of tokens that not all rows see were taken out
-        if (*(volatile unsigned*)&k.poison[i & 1][2 * half + part] & (~0u >> (32 - min(live, 32)))) l = NAN;
-      }
+      if (mine) l = NAN;
       // the row's maximum only where a score is above what P and O are relative to: all four threads of all 32 rows vote
       float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < 16; ++j) tops[j >> 2] = max3(tops[j >> 2], __uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1]));
-      float top = fmaxf(fmaxf(fmaf(tops[0], a.c, (float)ex[0]), fmaf(tops[1], a.c, (float)ex[1])), fmaxf(fmaf(tops[2], a.c, (float)ex[2]), fmaf(tops[3], a.c, (float)ex[3])));
+      float top = fmaxf(fmaf(fmaxf(tops[0], tops[1]), a.c, (float)ex[0]), fmaf(fmaxf(tops[2], tops[3]), a.c, (float)ex[1]));
       if (softmax_vote(rows32, t == s.t0 || top > m + kLag)) {
         k.best[2 * part + half][r] = top;
         softmax_barrier(rows32);
@@ -586,25 +628,29 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned char* q, u
       }
       const float off = kTop - (m == -INFINITY ? 0.f : m);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+      for (int g = 0; g < 2; ++g) {
         const f32x2 off2 = f2_splat(off + (float)ex[g]);
         f32x2 sum2[2] = {f2_splat(0.f), f2_splat(0.f)};
-        unsigned pw[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float e0, e1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[8 * g + 2 * j]), __uint_as_float(raw[8 * g + 2 * j + 1])), f2_splat(a.c), off2), e0, e1);
-          e0 = exp2_fast(e0);
-          e1 = exp2_fast(e1);
-          sum2[j & 1] = f2_add(sum2[j & 1], f2_pack(e0, e1));
-          if (MX8) {
-            const __half2 h = __floats2half2_rn(e0, e1);
-            pw[j] = *reinterpret_cast<const unsigned*>(&h);
-          } else {
-            pw[j] = pack_bf2(e0, e1);
+        for (int u = 0; u < 2; ++u) {
+          unsigned pw[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int at = 16 * g + 8 * u + 2 * j;
+            float e0, e1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[at]), __uint_as_float(raw[at + 1])), f2_splat(a.c), off2), e0, e1);
+            e0 = exp2_fast(e0);
+            e1 = exp2_fast(e1);
+            sum2[j & 1] = f2_add(sum2[j & 1], f2_pack(e0, e1));
+            if (MX8) {
+              const __half2 h = __floats2half2_rn(e0, e1);
+              pw[j] = *reinterpret_cast<const unsigned*>(&h);
+            } else {
+              pw[j] = pack_bf2(e0, e1);
+            }
           }
+          store16(p_mem + half * kQChunk + unit_at(r, part * 4 + 2 * g + u), make_uint4(pw[0], pw[1], pw[2], pw[3]));
         }
-        *reinterpret_cast<uint4*>(p_mem + half * kQChunk + unit_at(r, part * 4 + g)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
         float s0, s1;
         f2_unpack(f2_add(sum2[0], sum2[1]), s0, s1);
         l = fmaf(s0 + s1, __uint_as_float((unsigned)(127 - ex[g]) << 23), l);   // a token's weight itself, without its 2^E
@@ -647,20 +693,30 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned char* q, u
 }
 
 // ---- planning ---------------------------------------------------------------------------------------------------------------------------
-// The CTA's segments into the ring, and for the join the first and the last CTA of each row tile.
+// The CTA's segments and their tiles into the rings, and for the join the first and the last CTA of each row tile.
+__device__ __forceinline__ void plan_tile(Control& k, unsigned i, const Tile& t, int lane) {
+  if (i >= kTiles) wait(k, k.tile_empty[i % kTiles], (i / kTiles - 1) & 1, 200);
+  if (lane == 0) {
+    k.tile[i % kTiles] = t;
+    arrive(k.tile_full[i % kTiles]);
+  }
+  __syncwarp();
+}
 __device__ void plan(const AttnArgs& a, Control& k, int ptok, int lane) {
   long long left = k.left;
   int tile = k.first_tile, at = k.first_at;
+  unsigned i = 0;
   for (unsigned n = 0;; ++n) {
-    Segment s = {0, -1, 0, 0, 0, 0, nullptr};
+    Segment s = {0, -1, 0, 0, 0, 0};
+    const int* table = a.prefix_table;
     while (left > 0) {
-      s.b = -1; s.row0 = tile * kRows; s.tokens = ptok; s.table = a.prefix_table;
+      s.b = -1; s.row0 = tile * kRows; s.tokens = ptok;
       if (tile >= a.prefix_tiles) {
         s.b = (tile - a.prefix_tiles) / a.seq_tiles;
-        s.row0 = (tile - a.prefix_tiles - s.b * a.seq_tiles) * kRows;
-        s.tokens = s.b < a.B ? own_tokens(a, s.b) : 0;
-        s.table = a.block_table + (long long)s.b * a.max_pages;
         if (s.b >= a.B) break;
+        s.row0 = (tile - a.prefix_tiles - s.b * a.seq_tiles) * kRows;
+        s.tokens = own_tokens(a, s.b);
+        table = a.block_table + (long long)s.b * a.max_pages;
       }
       s.tile = tile;
       const int places = places_of(s.tokens), to = (int)min((long long)places, at + left);
@@ -676,13 +732,35 @@ __device__ void plan(const AttnArgs& a, Control& k, int ptok, int lane) {
       }
       s.t1 = 0;
     }
-    if (n >= kRing) wait(k, k.ring_empty[n % kRing], (n / kRing - 1) & 1, 1000);
+    if (n >= kRing) wait(k, k.ring_empty[n % kRing], (n / kRing - 1) & 1, 200);
     if (lane == 0) {
       k.ring[n % kRing] = s;
       arrive(k.ring_full[n % kRing]);
     }
     __syncwarp();
-    if (s.t1 == 0) return;
+    if (s.t1 == 0) {
+      plan_tile(k, i, Tile{{nullptr, nullptr}, {0, 0}, 0, 0}, lane);
+      return;
+    }
+    const int pages = (s.tokens + kPageTokens - 1) / kPageTokens;
+    int ids = 0;                                             // of page base + lane
+#pragma unroll 1
+    for (int t = s.t0; t < s.t1; ++t, ++i) {
+      const int off = (t - s.t0) * 2 % 32;
+      if (off == 0) ids = 2 * t + lane < pages ? __ldg(table + 2 * t + lane) : -1;
+      Tile w;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int id = __shfl_sync(0xffffffffu, ids, off + h);
+        const bool held = id >= 0 && id < a.pages;
+        w.page[h] = a.cache + (held ? id : 0) * a.page_stride;
+        w.tokens[h] = held ? max(0, min(kPageTokens, s.tokens - (2 * t + h) * kPageTokens)) : 0;
+      }
+      w.live = 1;
+      // steps of a sequence do not see all of its last S - 1 tokens: a value that is not finite must not reach the others through 0 * NaN
+      w.careful = s.b >= 0 && a.S > 1 && (t + 1) * kTile > s.tokens - (a.S - 1);
+      plan_tile(k, i, w, lane);
+    }
   }
 }
 
@@ -712,9 +790,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
     for (int u = 0; u < 5; ++u) init(k.full[u], kLoaders / 32);
 #pragma unroll 1
     for (int u = 0; u < 4; ++u) init(k.empty[u], 1);
-    init(k.s_full, 1); init(k.p_full, kSoftmax);
+    init(k.s_full, 1); init(k.s_read, kSoftmax / 32); init(k.p_full, kSoftmax);
 #pragma unroll 1
     for (int u = 0; u < kRing; ++u) { init(k.ring_full[u], 1); init(k.ring_empty[u], kReaders); }
+#pragma unroll 1
+    for (int u = 0; u < kTiles; ++u) { init(k.tile_full[u], 1); init(k.tile_empty[u], kLoaders / 32); }
     init(k.q_full, kSoftmax); init(k.o_free, kSoftmax);
     k.abort = 0;
 #pragma unroll 1
@@ -755,13 +835,13 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
   if (busy) {
     unsigned char *q = smem, *p = q + kSmemQ, *slots = p + kSmemP;
     if (warp < kSoftmax / 32) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-      softmax_tiles<MX8>(a, k, q, p, tid);
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+      softmax_tiles<MX8>(a, k, su(q), su(p), tid);
     } else if (warp < (kSoftmax + kLoaders) / 32) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-      Loader<MX8>(a, k, slots, tid - kSoftmax).run();
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+      Loader<MX8>(a, k, su(slots), tid - kSoftmax).run();
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
       if (warp == (kSoftmax + kLoaders) / 32) issue_tiles<MX8>(k, su(q), su(p), su(slots));
       else if (warp == (kSoftmax + kLoaders) / 32 + 3) plan(a, k, ptok, lane);
     }
@@ -892,7 +972,7 @@ K3G_API int k3g_latent_attn(const void* q, long long q_stride, const void* cache
   if (prefix_pages > 0) { K3G_REQUIRE_PTR(prefix_table); K3G_REQUIRE_PTR(prefix_len); }
   if (max_pages > 0) K3G_REQUIRE_PTR(block_table);
   const long long unit = cache_mx8 ? 1 : 2, page = cache_mx8 ? kMx8Page : 2 * kBf16Page;
-  const long long grain = cache_mx8 ? 32 : 16;
+  const long long grain = 32;
   K3G_REQUIRE(q_stride % 8 == 0 && layer_off * unit % grain == 0 && page_stride * unit % grain == 0 && (reinterpret_cast<uintptr_t>(cache) & (grain - 1)) == 0, K3G_EALIGN);
   K3G_REQUIRE(S > 0 && heads > 0 && q_stride >= (long long)heads * kRow && layer_off >= 0 && page_stride * unit >= layer_off * unit + page, K3G_ESHAPE);
   K3G_REQUIRE(B <= kMaxBatch && (long long)S * heads <= kMaxRowsPerSeq && prefix_pages <= (1 << 20) && max_pages <= (1 << 20), K3G_ELIMIT);

@@ -35,7 +35,7 @@ VERIFY = dict(target=P, target_stride=100, draft=P, draft_stride=100, ids=P, u=P
     ("k3g_latent_attn", ATTN, dict(q=None), -1), ("k3g_latent_attn", ATTN, dict(lens=None), -1), ("k3g_latent_attn", ATTN, dict(prefix_table=None), -1),
     ("k3g_latent_attn", ATTN, dict(prefix_len=None), -1), ("k3g_latent_attn", ATTN, dict(table=None), -1), ("k3g_latent_attn", ATTN, dict(workspace=None), -1),
     ("k3g_latent_attn", ATTN, dict(q=P + 2), -3), ("k3g_latent_attn", ATTN, dict(cache=P + 16), -3), ("k3g_latent_attn", ATTN, dict(q_stride=24 * ROW + 4), -3), ("k3g_latent_attn", ATTN, dict(workspace=P + 8), -3),
-    ("k3g_latent_attn", ATTN, dict(mx8=0, page_stride=PAGE * ROW + 4), -3), ("k3g_latent_attn", ATTN, dict(mx8=0, page_stride=PAGE * ROW - 8), -2),
+    ("k3g_latent_attn", ATTN, dict(mx8=0, page_stride=PAGE * ROW + 4), -3), ("k3g_latent_attn", ATTN, dict(mx8=0, page_stride=PAGE * ROW - 16), -2), ("k3g_latent_attn", ATTN, dict(mx8=0, layer_off=8, page_stride=2 * PAGE * ROW), -3),
     ("k3g_latent_attn", ATTN, dict(q_stride=23 * ROW), -2), ("k3g_latent_attn", ATTN, dict(S=0), -2), ("k3g_latent_attn", ATTN, dict(heads=0), -2),
     ("k3g_latent_attn", ATTN, dict(B=-1), -2), ("k3g_latent_attn", ATTN, dict(max_pages=-1), -2), ("k3g_latent_attn", ATTN, dict(B=4097), -5),
     ("k3g_latent_attn", ATTN, dict(S=32769, heads=1, q_stride=ROW), -5), ("k3g_latent_attn", ATTN, dict(max_pages=(1 << 20) + 1), -5),

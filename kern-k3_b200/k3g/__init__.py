@@ -67,13 +67,11 @@ for _name, _args in PROTOTYPES.items():
     _fn.argtypes = [_ctype(t) for t, _ in _args]
 
 
+# entry point -> (function, how many arguments, positions of the pointers): looked up once, a call is on the path of every launch
+_CALLS = {_n: (getattr(lib, _n), len(_a), tuple(_i for _i, (_t, _) in enumerate(_a) if "*" in _t)) for _n, _a in PROTOTYPES.items()}
+
+
 def _ptr(x):
-    if x is None:
-        return None
-    if hasattr(x, "data_ptr"):
-        return ctypes.c_void_p(x.data_ptr())
-    if isinstance(x, int):
-        return ctypes.c_void_p(x)
     if hasattr(x, "ctypes"):          # numpy array (host_ arguments)
         return ctypes.c_void_p(x.ctypes.data)
     if isinstance(x, (ctypes._SimpleCData, ctypes.Array)):   # host out-parameters
@@ -85,13 +83,19 @@ def _ptr(x):
 
 def raw(name, *args):
     """Call an entry point, return its integer status."""
-    spec = PROTOTYPES[name]
-    if len(args) != len(spec):
-        raise TypeError("%s takes %d arguments (%s), got %d" % (name, len(spec), ", ".join(n for _, n in spec), len(args)))
-    conv = []
-    for (ty, _), a in zip(spec, args):
-        conv.append(_ptr(a) if "*" in ty else a)
-    return getattr(lib, name)(*conv)
+    fn, count, pointers = _CALLS[name]
+    if len(args) != count:
+        raise TypeError("%s takes %d arguments (%s), got %d" % (name, count, ", ".join(n for _, n in PROTOTYPES[name]), len(args)))
+    conv = list(args)
+    for i in pointers:
+        a = conv[i]
+        if a is None or a.__class__ is int:
+            continue
+        try:
+            conv[i] = a.data_ptr()    # a tensor
+        except AttributeError:
+            conv[i] = a if isinstance(a, int) else _ptr(a)
+    return fn(*conv)
 
 
 def call(name, *args):

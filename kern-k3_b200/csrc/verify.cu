@@ -8,8 +8,13 @@
 //
 // Bound by HBM: one row of p and one of q per sequence (the other rows are touched at one entry each).  ONE CLUSTER PER
 // SEQUENCE, in one launch and without a workspace: each block sums a slice of the row, one contiguous segment per warp,
-// the segment sums are exchanged through distributed shared memory, and the one warp whose segment holds the drawn point
-// reads its segment again (from L2) and finds the token.
+// the segment sums are exchanged through distributed shared memory, and the block whose segment holds the drawn point
+// reads that segment again (from L2), a sixteenth for each warp, to find the token.  What stays beside the reading is the
+// chain ids -> p(x), q(x) -> rows -> exchange -> search, which takes 10 us however short the rows are.
+//
+// Four blocks of 512 threads on an SM, two loads of each row ahead: 64 sequences of 163840 entries with q (84 MB) take
+// 31 us from launch to end, 18 of them the chain and the launch.  Two blocks of 64 registers with four loads ahead take
+// 35 us (200 sequences: 94 against 70), three of 40 registers 35, and one warp for the search 5 us more.
 #include <cooperative_groups.h>
 
 #include "k3g_device.cuh"
@@ -20,6 +25,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kThreads = 512, kSegs = kThreads / 32, kMaxCluster = 8, kMaxSteps = 32;
+constexpr int kBatch = 2;
 
 struct Rows {                       // the row that is sampled from: weight(v) = p[v], or max(p[v] - q(v), 0)
   const float* p;
@@ -70,11 +76,46 @@ __device__ __forceinline__ double lane_scan(double x, int lane) {   // sum of th
   return x;
 }
 
+// Lane l has the sums of parts 4 l .. 4 l + 3, and with `upto` their running sum (`start` before the first).  The part in
+// which it passes `point`, else the last that weighs anything, -1 if none does; `base`: the running sum before it.
+__device__ __forceinline__ int part_of(const double (&part)[4], double upto, double point, int lane, double& base, double start = 0.0) {
+  double at = __shfl_up_sync(0xffffffffu, upto, 1);
+  if (lane == 0) at = start;
+  int hit = -1, top = -1;
+  double hit_base = 0.0, top_base = 0.0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (part[j] > 0.0) {
+      top = 4 * lane + j; top_base = at;
+      if (hit < 0 && at + part[j] > point) { hit = top; hit_base = at; }
+    }
+    at += part[j];
+  }
+  const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), tops = __ballot_sync(0xffffffffu, top >= 0);
+  const int from = hits ? __ffs(hits) - 1 : tops ? 31 - __clz(tops) : 0;
+  base = __shfl_sync(0xffffffffu, hits ? hit_base : top_base, from);
+  return __shfl_sync(0xffffffffu, hits ? hit : top, from);
+}
+
+// A function of its own: inlined at both places the kernel needs more than the 32 registers with which four blocks fit an SM.
 template <bool VEC>
-__device__ __forceinline__ double segment_sum(const Rows& r, int lo, int hi, int lane) {
+__device__ __noinline__ double segment_sum(const Rows r, int lo, int hi, int lane) {
   double s = 0.0;
+  int v = lo + 4 * lane;
+  if (VEC && r.q) {                                          // kBatch loads of each row are on their way before the first is used
+    for (; v + 128 * (kBatch - 1) + 4 <= hi; v += 128 * kBatch) {
+      float4 p[kBatch], q[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        p[j] = __ldg(reinterpret_cast<const float4*>(r.p + v + 128 * j));
+        q[j] = __ldg(reinterpret_cast<const float4*>(r.q + v + 128 * j));
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) s += (weight(p[j].x, q[j].x) + weight(p[j].y, q[j].y)) + (weight(p[j].z, q[j].z) + weight(p[j].w, q[j].w));
+    }
+  }
 #pragma unroll 4
-  for (int v = lo + 4 * lane; v < hi; v += 128) {
+  for (; v < hi; v += 128) {
     double w[4];
     weights4<VEC>(r, v, hi, w);
     s += (w[0] + w[1]) + (w[2] + w[3]);
@@ -111,7 +152,7 @@ __device__ __forceinline__ int segment_find(const Rows& r, int lo, int hi, doubl
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads) verify_draft_kernel(const float* __restrict__ target, long long target_stride,
+__global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const float* __restrict__ target, long long target_stride,
                                                                 const float* __restrict__ draft, long long draft_stride,
                                                                 const long long* __restrict__ ids, const float* __restrict__ u,
                                                                 int* __restrict__ accepted, long long* __restrict__ tokens, int S, int V,
@@ -160,24 +201,26 @@ __global__ void __launch_bounds__(kThreads) verify_draft_kernel(const float* __r
   }
   // the segment that holds the point: the first whose running sum passes it, else the last that weighs anything
   const double point = (double)u[(long long)b * (S + 1) + S] * total;
-  double base = __shfl_up_sync(0xffffffffu, upto, 1);
-  if (lane == 0) base = 0.0;
-  int hit = -1, top = -1;
-  double hit_base = 0.0, top_base = 0.0;
+  double base;
+  const int pick_seg = part_of(part, upto, point, lane, base);
+  if (rank != (pick_seg < 0 ? 0 : pick_seg / kSegs)) return;
+  int pick = -1;
+  bool mine = warp == 0;
+  if (pick_seg >= 0) {                                       // the same once more within the segment: a part of it for each warp
+    const int first = min(V, pick_seg * seg), last = min(V, first + seg), step = (seg / kSegs + 3) / 4 * 4;
+    const int from = min(last, first + warp * step), to = warp == kSegs - 1 ? last : min(last, from + step);
+    const double x = segment_sum<VEC>(r, from, to, lane);
+    if (lane == 0) s_sum[warp] = x;
+    __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (part[j] > 0.0) {
-      top = 4 * lane + j; top_base = base;
-      if (hit < 0 && base + part[j] > point) { hit = top; hit_base = base; }
-    }
-    base += part[j];
+    for (int j = 0; j < 4; ++j) part[j] = 4 * lane + j < kSegs ? s_sum[4 * lane + j] : 0.0;
+    upto = base + lane_scan((part[0] + part[1]) + (part[2] + part[3]), lane);
+    double sub_base;
+    const int sub = part_of(part, upto, point, lane, sub_base, base);
+    mine = warp == max(sub, 0);
+    if (mine) pick = segment_find<VEC>(r, from, to, sub_base, point, lane);
   }
-  const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), tops = __ballot_sync(0xffffffffu, top >= 0);
-  const int from = hits ? __ffs(hits) - 1 : tops ? 31 - __clz(tops) : 0;
-  const int pick_seg = __shfl_sync(0xffffffffu, hits ? hit : top, from);
-  base = __shfl_sync(0xffffffffu, hits ? hit_base : top_base, from);
-  if (pick_seg < 0 ? (rank == 0 && warp == 0) : pick_seg == rank * kSegs + warp) {
-    const int pick = pick_seg < 0 ? -1 : segment_find<VEC>(r, lo, hi, base, point, lane);
+  if (mine) {
     if (lane == 0) accepted[b] = kept;
     for (int i = lane; i <= S; i += 32)
       tokens[(long long)b * (S + 1) + i] = i < kept ? ids[(long long)b * S + i] : i == kept ? (long long)pick : -1ll;

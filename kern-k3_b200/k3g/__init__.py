@@ -105,8 +105,10 @@ def call(name, *args):
 
 
 def current_stream():
+    """Handle of torch's current stream on the current device."""
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw_stream(torch.cuda.current_device()) if raw_stream else torch.cuda.current_stream().cuda_stream
 
 
 def latent_attn_workspace(B, S, heads):

@@ -52,7 +52,7 @@ constexpr int kTmemS = 256, kTmemR = 320, kTmemQ = 384;
 constexpr int kLeastE = -80, kMostE = 120;                   // exponents of 16 tokens: sums of 2^-E stay in range
 constexpr float kLag = 4.f, kTop = 10.f;
 constexpr int kPartFloats = kRows * kLatent;                 // a part's outputs; its 64 (maximum, sum) pairs lie in a table of their own
-constexpr int kWaitLimit = 1 << 20, kRing = 4, kReaders = kSoftmax / 32 + 1, kTiles = 4;
+constexpr int kWaitLimit = 1 << 20, kRing = 4, kReaders = kSoftmax / 32 + 1, kTiles = 2;
 constexpr int kStart = 2;
 
 struct AttnArgs {
@@ -64,7 +64,7 @@ struct AttnArgs {
   int* status;                       // [kMaxCtas] 1: a wait of this CTA expired
   int2* spans;                       // [row tiles] first and last CTA of each (unwritten where there are no tokens)
   float2* sums;                      // [parts][64] (maximum in log2 units, sum)
-  float* parts;                      // [parts][64][512]
+  float* parts;                      // [parts][64 groups of 8 columns][64 rows][8]: what a warp writes at a time lies together
   int B, S, heads, prefix_tiles, seq_tiles, ctas;
   float c;                           // |scale| * log2(e), above 0 (scores are compared before they are scaled)
   int flip;                          // the scale is negative
@@ -467,59 +467,59 @@ __device__ __forceinline__ const __nv_bfloat16* query(const AttnArgs& a, const S
   const int step = at / a.heads;
   return a.q + ((s.b < 0 ? 0 : s.b * a.S) + step) * a.q_stride + (at - step * a.heads) * kRow;
 }
-// The latent columns of a segment's queries on their way into shared memory, four threads to a row; zeros where the tile has no row.
-__device__ __forceinline__ void fetch_q(const AttnArgs& a, const Segment& s, unsigned q, int tid) {
-  const int r = tid >> 2;
-  const unsigned char* src = reinterpret_cast<const unsigned char*>(query(a, s, r));
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const int unit = 4 * i + (tid & 3);
-    copy16(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7), src ? src + unit * 16 : reinterpret_cast<const unsigned char*>(a.q), src != nullptr);
-  }
-  copies_commit();
-}
-// The rope columns into tensor memory, by the first four warps (every row on both halves of the lanes).
-__device__ __forceinline__ void fetch_q_rope(const AttnArgs& a, const Segment& s, unsigned at, int r) {
-  const __nv_bfloat16* src = query(a, s, r);
-  unsigned v[32];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint4 x = src ? __ldg(reinterpret_cast<const uint4*>(src + kLatent) + i) : make_uint4(0u, 0u, 0u, 0u);
-    v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
-  }
-  tmem_st32(at, v);
-  tmem_wait_st();
-}
-// They have come: for MXFP8 pages made f16 where they lie, the row's largest element brought to 2^14 .. 2^15, each thread what it fetched.
+// A segment's queries.  Four threads to a row bring its latent columns into shared memory, zeros where the tile has no row: for bf16 pages
+// copied, for MXFP8 pages made f16, the row's largest element brought to 2^14 .. 2^15.  The rope columns go into tensor memory,
+// 32 of a row from each thread (each row on both halves of the lanes).
 template <bool MX8>
-__device__ __forceinline__ void q_ready(Control& k, unsigned q, unsigned n, int tid) {
-  copies_left<0>();
-  if (MX8) {
-    const int r = tid >> 2;
-    unsigned top = 0;
-#pragma unroll 4
-    for (int i = 0; i < 16; ++i) {
+__device__ __forceinline__ void fetch_q(const AttnArgs& a, Control& k, const Segment& s, unsigned n, unsigned q, unsigned rope_at, int tid) {
+  const int r = tid >> 2;
+  const __nv_bfloat16* src = query(a, s, r);
+  const uint4* from = reinterpret_cast<const uint4*>(src) + (tid & 3);
+  uint4 x[16];
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (MX8) {
+      x[i] = src ? __ldg(from + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
+    } else {
       const int unit = 4 * i + (tid & 3);
-      const uint4 x = load16(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7));
-      top = max(top, absmax8(V8{{x.x, x.y, x.z, x.w}}));
+      copy16(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7), reinterpret_cast<const unsigned char*>(src ? from + 4 * i : reinterpret_cast<const uint4*>(a.q)), src != nullptr);
     }
+  }
+  if (MX8) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, absmax8(V8{{x[i].x, x[i].y, x[i].z, x[i].w}}));
+  }
+  if (MX8) {
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e = (int)(top >> 7);                           // exponent field of the largest element; 0: a row of zeros (or of subnormals), 255: not finite
     const int shift = e == 0 || e == 255 ? 0 : max(e - 127 - 14, -120);   // q' = q * 2^-shift
     const float up = __uint_as_float((unsigned)(127 - shift) << 23);
     if ((tid & 3) == 0) k.row_shift[n & 1][r] = (signed char)shift;
-#pragma unroll 4
+    auto half = [&](unsigned w) {
+      const __half2 h = __floats2half2_rn(bf_lo(w) * up, bf_hi(w) * up);
+      return *reinterpret_cast<const unsigned*>(&h);
+    };
+#pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int unit = 4 * i + (tid & 3);
-      const unsigned at = q + (unit >> 3) * kQChunk + unit_at(r, unit & 7);
-      const uint4 x = load16(at);
-      auto half = [&](unsigned w) {
-        const __half2 h = __floats2half2_rn(bf_lo(w) * up, bf_hi(w) * up);
-        return *reinterpret_cast<const unsigned*>(&h);
-      };
-      store16(at, make_uint4(half(x.x), half(x.y), half(x.z), half(x.w)));
+      store16(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7), make_uint4(half(x[i].x), half(x[i].y), half(x[i].z), half(x[i].w)));
     }
+  }
+  const __nv_bfloat16* rope_src = query(a, s, tid & 63);
+  unsigned rope[16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 y = rope_src ? __ldg(reinterpret_cast<const uint4*>(rope_src + kLatent + (tid >> 7) * 32) + i) : make_uint4(0u, 0u, 0u, 0u);
+    rope[4 * i] = y.x; rope[4 * i + 1] = y.y; rope[4 * i + 2] = y.z; rope[4 * i + 3] = y.w;
+  }
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+               :: K3G_I8(rope, 0), K3G_I8(rope, 8), "r"(rope_at + (tid >> 7) * 16) : "memory");
+  tmem_wait_st();
+  if (!MX8) {
+    copies_commit();
+    copies_left<0>();
   }
   fence_async();
   fence_before();
@@ -548,9 +548,7 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigne
   {
     const Segment s = segment(k, 0, false);
     if (s.t1 == 0) return;
-    fetch_q(a, s, q, tid);
-    if (part == 0) fetch_q_rope(a, s, tq, r);
-    q_ready<MX8>(k, q, 0, tid);
+    fetch_q<MX8>(a, k, s, 0, q, tq, tid);
   }
   unsigned i = 0;
   for (unsigned n = 0;; ++n) {
@@ -661,11 +659,7 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigne
     }
     // the last product with this segment's queries is done: the next segment's take their place while P V goes on
     const Segment next = segment(k, n + 1, false);
-    if (next.t1 > 0) {
-      fetch_q(a, next, q, tid);
-      if (part == 0) fetch_q_rope(a, next, tq, r);
-      q_ready<MX8>(k, q, n + 1, tid);
-    }
+    if (next.t1 > 0) fetch_q<MX8>(a, k, next, n + 1, q, tq, tid);
     // this stretch's unnormalised outputs, maximum and sum
     wait(k, k.empty[3], (i - 1) & 1);
     fence_after();
@@ -675,7 +669,7 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigne
     softmax_barrier(rows32);
     if (half + part == 0 && live_row) a.sums[at * kRows + r] = make_float2(m, (k.best[0][r] + k.best[1][r]) + (k.best[2][r] + k.best[3][r]));
     softmax_barrier(rows32);                                 // the sums are read before a maximum takes their place
-    float* dst = a.parts + at * kPartFloats + r * kLatent + part * 256 + half * 64;
+    float* dst = a.parts + at * kPartFloats + ((part * 32 + half * 8) * kRows + r) * 8;
 #pragma unroll 1
     for (int c = 0; c < 128; c += 32) {
       unsigned v[32];
@@ -684,7 +678,7 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigne
       if (live_row) {
 #pragma unroll
         for (int j = 0; j < 32; j += 8)
-          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(dst + (c >> 6) * 128 + (c & 63) + j), K3G_I8(v, j) : "memory");
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(dst + ((c >> 6) * 16 + ((c & 63) + j) / 8) * (kRows * 8)), K3G_I8(v, j) : "memory");
       }
     }
     fence_before();
@@ -702,7 +696,10 @@ __device__ __forceinline__ void plan_tile(Control& k, unsigned i, const Tile& t,
   }
   __syncwarp();
 }
-__device__ void plan(const AttnArgs& a, Control& k, int ptok, int lane) {
+__device__ __forceinline__ void prefetch(const unsigned char* p, int bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p), "r"(bytes) : "memory");
+}
+__device__ void plan(const AttnArgs& a, Control& k, int ptok, int page_bytes, int lane) {
   long long left = k.left;
   int tile = k.first_tile, at = k.first_at;
   unsigned i = 0;
@@ -760,6 +757,8 @@ __device__ void plan(const AttnArgs& a, Control& k, int ptok, int lane) {
       // steps of a sequence do not see all of its last S - 1 tokens: a value that is not finite must not reach the others through 0 * NaN
       w.careful = s.b >= 0 && a.S > 1 && (t + 1) * kTile > s.tokens - (a.S - 1);
       plan_tile(k, i, w, lane);
+      // L2 has the pages before the loaders ask for them: a load that goes to HBM takes longer than the rest of a tile leaves it
+      if (lane < 2 && (lane ? w.tokens[1] : w.tokens[0])) prefetch(lane ? w.page[1] : w.page[0], page_bytes);
     }
   }
 }
@@ -808,10 +807,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
   fence_before();
   __syncthreads();
   fence_after();
-  long long before = prefix_places, total = prefix_places;
-#pragma unroll 1
-  for (int i = 0; i < kThreads / 32; ++i) { const long long v = k.scan[i]; if (i < warp) before += v; total += v; }
-  before += upto - mine;
+  long long at = lane < kThreads / 32 ? k.scan[lane] : 0, upto_warp = at;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto_warp, o);
+    if (lane >= o) upto_warp += v;
+  }
+  const long long total = prefix_places + __shfl_sync(0xffffffffu, upto_warp, 31);
+  long long before = prefix_places + __shfl_sync(0xffffffffu, upto_warp - at, warp) + upto - mine;
   const int ctas = (int)min((long long)gridDim.x, total);    // those with work: CTA i takes places total * i / ctas ..
   const bool busy = (int)blockIdx.x < ctas;
   if (busy) {
@@ -843,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
       if (warp == (kSoftmax + kLoaders) / 32) issue_tiles<MX8>(k, su(q), su(p), su(slots));
-      else if (warp == (kSoftmax + kLoaders) / 32 + 3) plan(a, k, ptok, lane);
+      else if (warp == (kSoftmax + kLoaders) / 32 + 3) plan(a, k, ptok, MX8 ? kMx8Page : 2 * kBf16Page, lane);
     }
   }
   fence_before();
@@ -853,66 +856,66 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
 }
 
 // ---- joining the parts of each row ------------------------------------------------------------------------------------------------------
-// GROUPS warps a row, two rows a block or one: lane j of a warp owns columns 128 x + 4 j .. + 3 (x = 0..3), warp g takes every GROUPS-th part.  Parts are
-// weighed by 2^(m - max m); the order of the sums depends on the lengths alone.
-constexpr int kJoinWarps = 8;
+// A team of four warps for four rows that follow one another, warp w its columns 128 w .. + 127: a lane has of one row 16 columns, and the eight lanes
+// that load together read 128 bytes that lie together when the rows lie in one tile.  GROUPS teams share the parts of their rows.
+// Parts are weighed by 2^(m - max m), the maximum a running one; the order of the sums depends on the lengths alone.
 template <int GROUPS>
-__global__ void __launch_bounds__(32 * kJoinWarps) latent_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas, int rows) {
-  __shared__ float4 s_out[GROUPS > 1 ? kJoinWarps : 1][128];
-  __shared__ float s_l[kJoinWarps];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = warp % GROUPS;
-  const int row = blockIdx.x * (kJoinWarps / GROUPS) + warp / GROUPS;
+__global__ void __launch_bounds__(128 * GROUPS) latent_attn_join_kernel(const __grid_constant__ AttnArgs a, int ctas, int rows) {
+  __shared__ float4 s_out[GROUPS > 1 ? GROUPS - 1 : 1][4][128];
+  __shared__ float2 s_sum[GROUPS > 1 ? GROUPS - 1 : 1][128];
+  const int tid = threadIdx.x, lane = tid & 31, quarter = (tid >> 5) & 3, g = tid >> 7, t = tid & 127;
+  const int row = blockIdx.x * 4 + ((lane >> 1) & 3);
   const bool there = row < rows;
   const int per_seq = a.S * a.heads, b = there ? row / per_seq : 0, in_seq = row - b * per_seq;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  int gave_up = 0;
-  for (int i = tid; i < ctas; i += 32 * kJoinWarps) gave_up |= a.status[i];
   const int len = __ldg(a.lens + b), ptok = prefix_tokens(a), own = own_tokens(a, b);
   const bool live = there && len >= 0;
+  // the parts: those of the row's tile against the prefix, then those against its own tokens; part (CTA, tile) has index CTA + tile
+  const int ptile = row / kRows, otile = a.prefix_tiles + b * a.seq_tiles + in_seq / kRows;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int gave_up = 0;
+  for (int i = tid; i < ctas; i += 128 * GROUPS) gave_up |= a.status[i];
+  const int2 ps = live && ptok ? a.spans[ptile] : make_int2(0, -1), os = live && own ? a.spans[otile] : make_int2(0, -1);
+  const int np = ps.y + 1 - ps.x, parts = np + os.y + 1 - os.x;
+  const int col = (quarter * 16 + (lane >> 3)) * (kRows * 8) + (lane & 1) * 4;   // of the lane's first columns within a part; the next 4 groups on
   float4 acc[4] = {};
-  float l = 0.f;
-  if (live) {
-    // the parts: those of the row's tile against the prefix, then those against its own tokens; part (CTA, tile) has index CTA + tile
-    const int ptile = row / kRows, otile = a.prefix_tiles + b * a.seq_tiles + in_seq / kRows;
-    const int2 ps = ptok ? a.spans[ptile] : make_int2(0, -1), os = own ? a.spans[otile] : make_int2(0, -1);
-    const int np = ps.y + 1 - ps.x, parts = np + os.y + 1 - os.x;
-    auto slot = [&](int i) { return i < np ? (long long)(ps.x + i + ptile) * kRows + row % kRows : (long long)(os.x + (i - np) + otile) * kRows + in_seq % kRows; };
-    float best = -INFINITY;
-    for (int i = lane; i < parts; i += 32) best = fmaxf(best, a.sums[slot(i)].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-    const float off = best == -INFINITY ? 0.f : best;
+  float l = 0.f, best = -INFINITY;
 #pragma unroll 2
-    for (int i = g; i < parts; i += GROUPS) {
-      const long long at = slot(i);
-      const float2 ml = a.sums[at];
-      float4 v[4];
+  for (int i = g; i < parts; i += GROUPS) {
+    const long long part = i < np ? ps.x + i + ptile : os.x + (i - np) + otile;
+    const int r = (i < np ? row : in_seq) % kRows;
+    const float2 ml = a.sums[part * kRows + r];
+    float4 v[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) v[x] = __ldcs(reinterpret_cast<const float4*>(a.parts + at * kLatent) + 32 * x + lane);
-      const float f = exp2f(ml.x - off);
-      l = fmaf(ml.y, f, l);
+    for (int x = 0; x < 4; ++x) v[x] = __ldcs(reinterpret_cast<const float4*>(a.parts + part * kPartFloats + col + r * 8 + x * 4 * (kRows * 8)));
+    const float top = fmaxf(best, ml.x), off = top == -INFINITY ? 0.f : top, f0 = exp2f(best - off), f = exp2f(ml.x - off);
+    best = top;
+    l = fmaf(ml.y, f, l * f0);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        acc[x].x = fmaf(v[x].x, f, acc[x].x); acc[x].y = fmaf(v[x].y, f, acc[x].y);
-        acc[x].z = fmaf(v[x].z, f, acc[x].z); acc[x].w = fmaf(v[x].w, f, acc[x].w);
-      }
+    for (int x = 0; x < 4; ++x) {
+      acc[x].x = fmaf(v[x].x, f, acc[x].x * f0); acc[x].y = fmaf(v[x].y, f, acc[x].y * f0);
+      acc[x].z = fmaf(v[x].z, f, acc[x].z * f0); acc[x].w = fmaf(v[x].w, f, acc[x].w * f0);
     }
   }
-  if (GROUPS > 1) {
+  if (GROUPS > 1 && g > 0) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) s_out[warp][32 * x + lane] = acc[x];
-    if (lane == 0) s_l[warp] = l;
+    for (int x = 0; x < 4; ++x) s_out[g - 1][x][t] = acc[x];
+    s_sum[g - 1][t] = make_float2(best, l);
   }
   const bool failed = __syncthreads_or(gave_up);
   if (!live || g > 0) return;                                // no sequence: left as it was
   if (GROUPS > 1) {
-    for (int i = 1; i < GROUPS; ++i) {
+#pragma unroll
+    for (int i = 0; i < GROUPS - 1; ++i) {
+      const float2 ml = s_sum[i][t];
+      const float top = fmaxf(best, ml.x), off = top == -INFINITY ? 0.f : top, f0 = exp2f(best - off), f = exp2f(ml.x - off);
+      best = top;
+      l = fmaf(ml.y, f, l * f0);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const float4 v = s_out[warp + i][32 * x + lane];
-        acc[x].x += v.x; acc[x].y += v.y; acc[x].z += v.z; acc[x].w += v.w;
+        const float4 v = s_out[i][x][t];
+        acc[x].x = fmaf(v.x, f, acc[x].x * f0); acc[x].y = fmaf(v.y, f, acc[x].y * f0);
+        acc[x].z = fmaf(v.z, f, acc[x].z * f0); acc[x].w = fmaf(v.w, f, acc[x].w * f0);
       }
-      l += s_l[warp + i];
     }
   }
   // a sum of exactly 0 has seen no token; NaN stays NaN; a call whose kernel gave up a wait has no result
@@ -921,7 +924,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) latent_attn_join_kernel(const
   for (int x = 0; x < 4; ++x) {
     uint2 w = make_uint2(pack_bf2(acc[x].x * f, acc[x].y * f), pack_bf2(acc[x].z * f, acc[x].w * f));
     if (l == 0.f && !failed) w = make_uint2(0u, 0u);
-    *reinterpret_cast<uint2*>(a.out + (long long)row * kLatent + 128 * x + 4 * lane) = w;
+    *reinterpret_cast<uint2*>(a.out + (long long)row * kLatent + (quarter * 16 + (lane >> 3) + 4 * x) * 8 + (lane & 1) * 4) = w;
   }
 }
 
@@ -941,9 +944,8 @@ Space space_of(int B, int S, int heads) {
 
 template <int GROUPS>
 cudaError_t launch_join(const AttnArgs& a, int ctas, int rows, cudaStream_t stream) {
-  constexpr int per = kJoinWarps / GROUPS;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((rows - 1) / per + 1), 1, 1); cfg.blockDim = dim3(32 * kJoinWarps, 1, 1); cfg.stream = stream;
+  cfg.gridDim = dim3((unsigned)((rows - 1) / 4 + 1), 1, 1); cfg.blockDim = dim3(128 * GROUPS, 1, 1); cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -994,9 +996,9 @@ K3G_API int k3g_latent_attn(const void* q, long long q_stride, const void* cache
   kernel<<<ctas, kThreads, kSmem, k3g_stream(stream)>>>(a);
   const int rc = k3g_launch_status();
   if (rc != K3G_OK) return rc;
-  // Few rows mean many parts for each: several warps share them (a card's 148 SMs hold about 1200 such warps at once and more).
+  // Few rows mean many parts for each: several teams share them.
   const int n = (int)rows;
-  e = n <= 148 ? launch_join<8>(a, ctas, n, k3g_stream(stream)) : n <= 1184 ? launch_join<4>(a, ctas, n, k3g_stream(stream)) : launch_join<1>(a, ctas, n, k3g_stream(stream));
+  e = n <= 1184 ? launch_join<4>(a, ctas, n, k3g_stream(stream)) : n <= 2368 ? launch_join<2>(a, ctas, n, k3g_stream(stream)) : launch_join<1>(a, ctas, n, k3g_stream(stream));
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   return k3g_launch_status();
 }

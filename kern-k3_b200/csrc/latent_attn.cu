@@ -838,10 +838,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
   if (busy) {
     unsigned char *q = smem, *p = q + kSmemQ, *slots = p + kSmemP;
     if (warp < kSoftmax / 32) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
       softmax_tiles<MX8>(a, k, su(q), su(p), tid);
     } else if (warp < (kSoftmax + kLoaders) / 32) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
       Loader<MX8>(a, k, su(slots), tid - kSoftmax).run();
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");

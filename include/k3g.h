@@ -389,10 +389,11 @@ int k3g_latent_gather(const void* slab, const void* block_table, long long page_
 
 /* ---- decoding with drafts over the latent cache (no counterpart in the reference, which only prefills) ---------- */
 /* The cache is paged as k3g_mla_prep writes it: pages of 64 tokens, a page table per sequence, `layer_off` the layer's place in
- * a page.  bf16 pages are 64 rows of 576 (512 latent columns, 64 rope columns); offsets and strides in elements (multiples of 16 here).  MXFP8 pages
- * are 41984 bytes in three planes -- 64 x 512 E4M3 codes, 64 x 64 bf16 (the rope columns as they are), 64 x 16 UE8M0 scale bytes --
- * 656 bytes a token instead of 1152; offsets and strides in bytes, multiples of 32, and the cache 32-byte aligned.  `pages` is the number of pages the cache
- * holds: a table entry outside [0, pages) is never read, and neither is one behind the last token of its sequence. */
+ * a page.  bf16 pages are 64 rows of 576 (512 latent columns, 64 rope columns); offsets and strides in elements (multiples of
+ * 16 here).  MXFP8 pages are 41984 bytes in three planes -- 64 x 512 E4M3 codes, 64 x 64 bf16 (the rope columns as they are),
+ * 64 x 16 UE8M0 scale bytes -- 656 bytes a token instead of 1152; offsets and strides in bytes, multiples of 32.  The cache
+ * is 32-byte aligned.  `pages` is the number of pages the cache holds: a table entry outside [0, pages) is never
+ * followed, and none behind the last token of its sequence is read. */
 
 /* Quantise T latent rows (576 bf16, `row_stride` elements apart, a multiple of 8) and append them: row t goes to slot
  * slot_mapping[t] (i64: page * 64 + row; a slot outside [0, 64 * pages) is skipped).  Codes and scales are k3g_moe_quant's for the
@@ -413,12 +414,13 @@ int k3g_latent_mx8_gather(const void* cache, const void* block_table, long long 
  * tables' capacity are cut to it.  q [B, S, heads, 576] bf16, q_stride elements (a multiple of 8) from one step to the next; out
  * [B, S, heads, 512] bf16.
  *   - lens[b] < 0: no sequence (a padded batch); its rows of out are left as they were.
- *   - a row that sees no token is zero; one that sees a NaN or an infinity is NaN, the others are not touched by it; what lies
- *     behind the last token of a page is not used.
+ *   - a row that sees no token is zero.  One that sees a NaN, or a score of +infinity, is NaN; a token whose score is -infinity
+ *     weighs nothing, but among the tokens that not all steps see (and those in one tile with them) an infinite value makes the
+ *     rows that see it NaN.  Rows that do not see it are not touched by it, and what lies behind a page's last token is not used.
  *   - prefix_pages = 0 / max_pages = 0: no prefix / no own tokens (the tables, and prefix_len, may be null).
  *   - workspace: 16-byte aligned device memory of k3g_latent_attn_workspace bytes (else K3G_EWORKSPACE), used by one call at a time:
  *     calls that may overlap, and captured graphs that may run together, need one each.  Its content need not be kept.
- * B <= 4096, S * heads <= 32768, prefix_pages and max_pages <= 2^20 (K3G_ELIMIT). */
+ * B <= 4096, S * heads <= 32768, prefix_pages and max_pages <= 2^20 (K3G_ELIMIT); scale finite (K3G_ERANGE). */
 int k3g_latent_attn(const void* q, long long q_stride, const void* cache, int cache_mx8, long long layer_off, long long page_stride,
                     long long pages, const void* prefix_table, const void* prefix_len, int prefix_pages, const void* block_table,
                     const void* lens, int max_pages, void* out, void* workspace, long long workspace_bytes, int B, int S, int heads,
@@ -432,9 +434,9 @@ int k3g_latent_attn_workspace(int B, int S, int heads, long long* host_bytes);
  * u [B, S + 1] f32 in [0, 1).  Draft i is kept while u[b, i] * q_i(ids[b, i]) < p_i(ids[b, i]); an id outside [0, V) ends the
  * sequence's drafts.  One more token follows the kept ones: at a draft turned down the first v whose running sum of max(p - q, 0)
  * exceeds u[b, S] times the whole sum, else (all kept, or p <= q everywhere) the same of p; sums in 64 bits, rows need not be
- * normalised, NaN, negative and infinite weights count as 0.  accepted [B] i32 = drafts kept; tokens [B, S + 1] i64 = the kept drafts, the token
- * that follows (-1 if its row weighs nothing), then -1.  S <= 32, V <= 2^30, B <= 2^24.  Rows with strides that are multiples of 4 are
- * read 16 bytes at a time. */
+ * normalised, NaN, negative and infinite weights count as 0.  accepted [B] i32 = drafts kept; tokens [B, S + 1] i64 = the kept
+ * drafts, the token that follows (-1 if its row weighs nothing), then -1.  S <= 32, V <= 2^30, B <= 2^24.  Rows with strides that
+ * are multiples of 4 are read 16 bytes at a time. */
 int k3g_verify_draft(const void* target, long long target_stride, const void* draft, long long draft_stride, const void* ids, const void* u,
                      void* accepted, void* tokens, int B, int S, int V, void* stream);
 

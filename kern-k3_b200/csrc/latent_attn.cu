@@ -5,12 +5,11 @@
 // key (576 columns) and value (its first 512) at once, so a tile of tokens is loaded once and used by two products.
 //
 // Work.  All rows (b, s, h) in tiles of 64 against the prefix, and each sequence's rows in tiles of 64 against its own
-// tokens, in tiles of 128 tokens (two pages): every (row tile, token tile) pair costs the same, and a row tile about kStart pairs more (its
-// queries in, its outputs out), so the pairs are laid in one line, row tile by row tile, kStart empty places before each, and each CTA
-// takes an equal stretch, whatever the lengths are.  A stretch that covers a part of a row tile
-// leaves an unnormalised f32 output with its maximum and sum in the workspace (one pass over the tokens, running maximum and
-// sum in 32 bits), and a second, dependent launch joins the parts of each row.  Lengths and tables are read on the device:
-// a captured graph follows them.  Nothing is accumulated by atomics: the same inputs give the same bits.
+// tokens, in tiles of 128 tokens (two pages).  Every (row tile, token tile) pair costs the same, 4 us, and a row tile about as much again
+// (its queries in, its outputs out): the pairs are laid in one line, row tile by row tile, kStart empty places before each, and each CTA takes an equal
+// stretch, whatever the lengths are.  A stretch that covers a part of a row tile leaves an unnormalised f32 output with its maximum and sum in the
+// workspace (one pass over the tokens, running maximum and sum in 32 bits), and a second, dependent launch joins the parts of each row.
+// Lengths and tables are read on the device: a captured graph follows them.  Nothing is accumulated by atomics: the same inputs give the same bits.
 //
 // One CTA per SM, warps with fixed roles, one token tile after another:
 //   1 planning warp  this CTA's stretches, one after another, and the pages of their tiles, into rings that the others read;
@@ -20,9 +19,17 @@
 //   8 softmax warps  S from tensor memory, running maximum, P = 2^(S - m) rounded to 16 bits into shared memory; O scaled, read and written out.
 // Why M = 64: a 128-row O of 512 columns fills the whole tensor memory and leaves no room for S.  The weight-stationary form puts
 // a 64-row tile on all 128 lanes and reaches 48 cycles per 64 x 128 x 16 step, the plain form 64 (measured; 32 would be full rate).
-// Why 128 tokens: a 64 x 64 x 16 step costs 44 cycles.  What bounds a tile is shared memory (operands of both products, the loaders' stores: 0.5 MB), so
-// pages of 64 tokens in two buffers, which let all roles work at once, took longer (2.3 against x us a tile).  O is made in four products of 128
-// columns: a pair of chunks is refilled as soon as its quarter of P V is done.  The queries' rope columns lie in tensor memory, which makes room for P.
+// Why 128 tokens: a 64 x 64 x 16 step costs 44 cycles.  Tiles of one page in two buffers, which let all roles work at once, took 425 us where this takes
+// 340 (below).  O is made in four products of 128 columns: a pair of chunks is refilled as soon as its quarter of P V is done.
+// The queries' rope columns lie in tensor memory, which makes room for P.
+//
+// What bounds it.  With few rows the cache's bytes, but only where the lengths hide the 20 us that a call's start, end and join take; with many rows, by the formulas,
+// the tensor cores (640 flops a byte for 64 rows).  What a pair waits for in fact is shared memory: a 64 x 128 x 16 step reads 6 KB of it, which is the 48
+// cycles, and with the loaders' stores (147 KB), their loads (84 KB at 64 bytes a clock) and P a pair needs 5900 cycles of it; it takes 7000.
+// More loader warps gain nothing for that reason (16 instead of 8: 351 us).
+// Measured: 8 x 96 rows against 131072 MXFP8 tokens 340 us (630 TFLOP/s, 38% of a dense bf16 product), 48 x 4 x 24 rows against 16384 and their own
+// 512 272 us, 32 x 24 rows against 8229 and 1024 49 us, 64 x 12 rows against their own 4096 49 us (1.8 TB/s), 16 x 2 x 48 rows against bf16
+// pages 57 us, one sequence of 500 tokens 16.5 us.
 //
 // Types.  bf16 pages are multiplied as bf16.  MXFP8 codes become f16, not bf16: one conversion and one product for two codes, a third of what bf16
 // takes (which has no conversion from E4M3), and the loaders' instructions are what a tile waits for.  f16 has the bits (a code has four), but not the
@@ -50,10 +57,10 @@ constexpr int kSmemQ = 8 * kQChunk, kSmemP = 2 * kQChunk, kSmemK = 9 * kChunk, k
 // half), the rope columns' part of S 320..383 (MXFP8), the queries' rope columns 384..415 (the same on both halves)
 constexpr int kTmemS = 256, kTmemR = 320, kTmemQ = 384;
 constexpr int kLeastE = -80, kMostE = 120;                   // exponents of 16 tokens: sums of 2^-E stay in range
-constexpr float kLag = 4.f, kTop = 10.f;
+constexpr float kLag = 4.f, kTop = 10.f;                     // the long document above 340 us, with a lag of 0 (O rescaled for every new maximum) 359
 constexpr int kPartFloats = kRows * kLatent;                 // a part's outputs; its 64 (maximum, sum) pairs lie in a table of their own
 constexpr int kWaitLimit = 1 << 20, kRing = 4, kReaders = kSoftmax / 32 + 1, kTiles = 2;
-constexpr int kStart = 2;
+constexpr int kStart = 2;                                     // the drafted tokens above 272 us, with 1 336, with 4 283
 
 struct AttnArgs {
   const __nv_bfloat16* q; long long q_stride;
@@ -757,7 +764,7 @@ __device__ void plan(const AttnArgs& a, Control& k, int ptok, int page_bytes, in
       // steps of a sequence do not see all of its last S - 1 tokens: a value that is not finite must not reach the others through 0 * NaN
       w.careful = s.b >= 0 && a.S > 1 && (t + 1) * kTile > s.tokens - (a.S - 1);
       plan_tile(k, i, w, lane);
-      // L2 has the pages before the loaders ask for them: a load that goes to HBM takes longer than the rest of a tile leaves it
+      // L2 has the pages before the loaders ask for them (two or three tiles ahead: 340 us for the long document, without it 346)
       if (lane < 2 && (lane ? w.tokens[1] : w.tokens[0])) prefetch(lane ? w.page[1] : w.page[0], page_bytes);
     }
   }
@@ -978,6 +985,7 @@ K3G_API int k3g_latent_attn(const void* q, long long q_stride, const void* cache
   K3G_REQUIRE(q_stride % 8 == 0 && layer_off * unit % grain == 0 && page_stride * unit % grain == 0 && (reinterpret_cast<uintptr_t>(cache) & (grain - 1)) == 0, K3G_EALIGN);
   K3G_REQUIRE(S > 0 && heads > 0 && q_stride >= (long long)heads * kRow && layer_off >= 0 && page_stride * unit >= layer_off * unit + page, K3G_ESHAPE);
   K3G_REQUIRE(B <= kMaxBatch && (long long)S * heads <= kMaxRowsPerSeq && prefix_pages <= (1 << 20) && max_pages <= (1 << 20), K3G_ELIMIT);
+  K3G_REQUIRE(scale - scale == 0.f, K3G_ERANGE);             // finite
   const Space sp = space_of(B, S, heads);
   K3G_REQUIRE(workspace_bytes >= sp.bytes, K3G_EWORKSPACE);
   int dev = 0, sms = 0;

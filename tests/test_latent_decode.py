@@ -192,6 +192,13 @@ def test_attn_many_tokens_split_over_the_card(k3g, dev, mx8):
     Case(dev, 2, 1, 24, 20000, [70, 3], mx8=mx8, seed=2).check(k3g)
 
 
+@pytest.mark.parametrize("mx8", [True, False])
+@pytest.mark.parametrize("B,S,heads", [(50, 3, 9), (101, 5, 5), (49, 1, 24)])
+def test_attn_rows_joined_by_one_two_and_four_teams(k3g, dev, mx8, B, S, heads):
+    """Row counts on either side of the join's borders, and sequences whose rows do not begin at multiples of four."""
+    Case(dev, B, S, heads, 1000, [S + (i * 29) % 150 for i in range(B)], mx8=mx8, seed=31).check(k3g)
+
+
 def test_attn_many_rows(k3g, dev):
     """More row tiles than SMs, with sequences that begin inside a tile."""
     Case(dev, 150, 3, 24, 130, [3 + (i * 37) % 100 for i in range(150)], seed=3).check(k3g)

@@ -39,6 +39,8 @@ VERIFY = dict(target=P, target_stride=100, draft=P, draft_stride=100, ids=P, u=P
     ("k3g_latent_attn", ATTN, dict(q_stride=23 * ROW), -2), ("k3g_latent_attn", ATTN, dict(S=0), -2), ("k3g_latent_attn", ATTN, dict(heads=0), -2),
     ("k3g_latent_attn", ATTN, dict(B=-1), -2), ("k3g_latent_attn", ATTN, dict(max_pages=-1), -2), ("k3g_latent_attn", ATTN, dict(B=4097), -5),
     ("k3g_latent_attn", ATTN, dict(S=32769, heads=1, q_stride=ROW), -5), ("k3g_latent_attn", ATTN, dict(max_pages=(1 << 20) + 1), -5),
+    ("k3g_latent_attn", ATTN, dict(prefix_pages=(1 << 20) + 1), -5), ("k3g_latent_attn", ATTN, dict(prefix_pages=-1), -2), ("k3g_latent_attn", ATTN, dict(pages=1 << 31), -2),
+    ("k3g_latent_attn", ATTN, dict(scale=float("nan")), -4), ("k3g_latent_attn", ATTN, dict(scale=float("-inf")), -4), ("k3g_latent_attn", ATTN, dict(scale=3e38, bytes=0), -6),
     ("k3g_latent_attn", ATTN, dict(bytes=0), -6), ("k3g_latent_attn", ATTN, dict(B=0), 0),
     ("k3g_verify_draft", VERIFY, dict(target=None), -1), ("k3g_verify_draft", VERIFY, dict(ids=None), -1), ("k3g_verify_draft", VERIFY, dict(target=P + 4), -3),
     ("k3g_verify_draft", VERIFY, dict(draft=P + 4), -3), ("k3g_verify_draft", VERIFY, dict(target_stride=99), -2), ("k3g_verify_draft", VERIFY, dict(draft_stride=99), -2),

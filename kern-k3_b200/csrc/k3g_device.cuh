@@ -2,8 +2,8 @@
 //
 // Everything here is register-level: 16-byte global accesses with cache hints, bf16 pair
 // packing, the E4M3 / UE8M0 (MXFP8) conversions, fixed-order warp reductions and the
-// IEEE-only exp used where an integer decision depends on a transcendental.  No kernel in
-// this library is a dense contraction, so there is no tensor-core code.
+// IEEE-only exp used where an integer decision depends on a transcendental.  The one dense
+// contraction of this library, latent_attn.cu, keeps its tensor-core code to itself.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>

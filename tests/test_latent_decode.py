@@ -148,11 +148,11 @@ class Case:
         self.ws = torch.empty(k3g.latent_attn_workspace(self.B, self.S, self.heads), dtype=torch.uint8, device=d)
         return self
 
-    def call(self, k3g, stream=None, out=None, ws=None):
+    def call(self, k3g, out=None, ws=None):
         out, ws = self.out if out is None else out, self.ws if ws is None else ws
         k3g.call("k3g_latent_attn", self.d_q, self.q.shape[2], self.d_cache, int(self.mx8), self.off, self.stride, self.pages, self.d_pt, self.d_pl,
                  self.prefix_pages, self.d_tables, self.d_lens, self.max_pages, out, ws, ws.numel(), self.B, self.S, self.heads, self.scale,
-                 k3g.current_stream() if stream is None else stream)
+                 k3g.current_stream())
 
     def oracle(self):
         read = mx8_rows if self.mx8 else bf16_rows
@@ -350,7 +350,8 @@ def test_attn_same_bits_every_time_and_on_two_streams_at_once(k3g, dev):
     torch.cuda.synchronize()
     for _ in range(5):
         for st, o, w in zip(streams, outs, spaces):
-            c.call(k3g, stream=st.cuda_stream, out=o, ws=w)
+            with torch.cuda.stream(st):
+                c.call(k3g, out=o, ws=w)
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o.view(torch.int16), first.view(torch.int16))

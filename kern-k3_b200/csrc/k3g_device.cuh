@@ -11,6 +11,13 @@
 
 namespace k3g {
 
+// For kernels launched by k3g_launch_behind, before anything is read or written that another launch writes or reads: wait until what
+// came before has ended, then let the next launch begin (it waits in turn).
+__device__ __forceinline__ void follow_launch() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 struct V8 { unsigned w[4]; };   // eight bf16 = one 16-byte vector
 
 // ---- global memory, 16 bytes at a time -------------------------------------------------

@@ -776,21 +776,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<unsigned long long>(raw) + 1023) & ~1023ull);
   __shared__ Control k;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // the line: places of sequences b0 .. b1 by this thread, then a scan over the block
-  const int ptok = prefix_tokens(a);
-  const long long prefix_places = (long long)a.prefix_tiles * places_of(ptok);
-  const int per = (a.B + kThreads - 1) / kThreads, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
-  long long mine = 0;
-#pragma unroll 1
-  for (int b = b0; b < b1; ++b) mine += a.seq_tiles * places_of(own_tokens(a, b));
-  long long upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) k.scan[warp] = upto;
   if (tid == 0) {
     auto init = [](unsigned long long& bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(su(&bar)), "r"(n)); };
     for (int u = 0; u < 5; ++u) init(k.full[u], kLoaders / 32);
@@ -810,6 +795,21 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(su(&k.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  follow_launch();                                           // what came before this launch is done; the join may begin, and waits for this one
+  // the line: places of sequences b0 .. b1 by this thread, then a scan over the block
+  const int ptok = prefix_tokens(a);
+  const long long prefix_places = (long long)a.prefix_tiles * places_of(ptok);
+  const int per = (a.B + kThreads - 1) / kThreads, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+  long long mine = 0;
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) mine += a.seq_tiles * places_of(own_tokens(a, b));
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) k.scan[warp] = upto;
   fence_async();
   fence_before();
   __syncthreads();
@@ -878,7 +878,7 @@ __global__ void __launch_bounds__(128 * GROUPS) latent_attn_join_kernel(const __
   const bool live = there && len >= 0;
   // the parts: those of the row's tile against the prefix, then those against its own tokens; part (CTA, tile) has index CTA + tile
   const int ptile = row / kRows, otile = a.prefix_tiles + b * a.seq_tiles + in_seq / kRows;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  follow_launch();
   int gave_up = 0;
   for (int i = tid; i < ctas; i += 128 * GROUPS) gave_up |= a.status[i];
   const int2 ps = live && ptok ? a.spans[ptile] : make_int2(0, -1), os = live && own ? a.spans[otile] : make_int2(0, -1);
@@ -951,13 +951,7 @@ Space space_of(int B, int S, int heads) {
 
 template <int GROUPS>
 cudaError_t launch_join(const AttnArgs& a, int ctas, int rows, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((rows - 1) / 4 + 1), 1, 1); cfg.blockDim = dim3(128 * GROUPS, 1, 1); cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at; cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, latent_attn_join_kernel<GROUPS>, a, ctas, rows);
+  return k3g_launch_behind(latent_attn_join_kernel<GROUPS>, (unsigned)((rows - 1) / 4 + 1), 128 * GROUPS, 0, 1, stream, a, ctas, rows);
 }
 
 }  // namespace
@@ -1001,9 +995,8 @@ K3G_API int k3g_latent_attn(const void* q, long long q_stride, const void* cache
                 (const int*)prefix_table, (const int*)prefix_len, prefix_pages, (const int*)block_table, (const int*)lens, max_pages,
                 (__nv_bfloat16*)out, (int*)ws, (int2*)(ws + sp.spans), (float2*)(ws + sp.sums), (float*)(ws + sp.parts),
                 B, S, heads, (int)((rows + kRows - 1) / kRows), (S * heads + kRows - 1) / kRows, ctas, fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-30f), scale < 0.f};
-  kernel<<<ctas, kThreads, kSmem, k3g_stream(stream)>>>(a);
-  const int rc = k3g_launch_status();
-  if (rc != K3G_OK) return rc;
+  e = k3g_launch_behind(kernel, (unsigned)ctas, kThreads, kSmem, 1, k3g_stream(stream), a);
+  if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   // Few rows mean many parts for each: several teams share them.
   const int n = (int)rows;
   e = n <= 1184 ? launch_join<4>(a, ctas, n, k3g_stream(stream)) : n <= 2368 ? launch_join<2>(a, ctas, n, k3g_stream(stream)) : launch_join<1>(a, ctas, n, k3g_stream(stream));

@@ -25,6 +25,7 @@ __global__ void __launch_bounds__(32 * kWarps) latent_mx8_store_kernel(const __n
                                                                        long long slots, int T) {
   const int lane = threadIdx.x & 31;
   const long long t = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  follow_launch();
   if (t >= T) return;
   const long long slot = __ldg(slot_mapping + t);
   const __nv_bfloat16* row = rows + t * row_stride;
@@ -50,6 +51,7 @@ __global__ void __launch_bounds__(32 * kWarps) latent_mx8_gather_kernel(const un
                                                                         long long page_stride, long long pages, const int* __restrict__ lens,
                                                                         __nv_bfloat16* __restrict__ out, int n) {
   const int lane = threadIdx.x & 31;
+  follow_launch();
   const int len = lens[0];
   const long long t = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (t >= n) return;
@@ -82,8 +84,9 @@ K3G_API int k3g_latent_mx8_store(const void* rows, long long row_stride, const v
   K3G_REQUIRE(T >= 0 && pages >= 0 && pages < (1ll << 31), K3G_ESHAPE);
   if (T == 0) return K3G_OK;
   K3G_REQUIRE(row_stride >= kRow && layer_off >= 0 && page_stride >= layer_off + kMx8Page, K3G_ESHAPE);
-  latent_mx8_store_kernel<<<(T - 1) / kWarps + 1, 32 * kWarps, 0, k3g_stream(stream)>>>(
-      (const __nv_bfloat16*)rows, row_stride, (const long long*)slot_mapping, (unsigned char*)cache + layer_off, page_stride, pages * kPageTokens, T);
+  const cudaError_t e = k3g_launch_behind(latent_mx8_store_kernel, (T - 1) / kWarps + 1, 32 * kWarps, 0, 1, k3g_stream(stream), (const __nv_bfloat16*)rows, row_stride,
+                                          (const long long*)slot_mapping, (unsigned char*)cache + layer_off, page_stride, pages * kPageTokens, T);
+  if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   return k3g_launch_status();
 }
 
@@ -95,7 +98,8 @@ K3G_API int k3g_latent_mx8_gather(const void* cache, const void* block_table, lo
   K3G_REQUIRE(n >= 0 && pages >= 0 && pages < (1ll << 31), K3G_ESHAPE);
   if (n == 0) return K3G_OK;
   K3G_REQUIRE(layer_off >= 0 && page_stride >= layer_off + kMx8Page, K3G_ESHAPE);
-  latent_mx8_gather_kernel<<<(n - 1) / kWarps + 1, 32 * kWarps, 0, k3g_stream(stream)>>>(
-      (const unsigned char*)cache + layer_off, (const int*)block_table, page_stride, pages, (const int*)lens, (__nv_bfloat16*)out, n);
+  const cudaError_t e = k3g_launch_behind(latent_mx8_gather_kernel, (n - 1) / kWarps + 1, 32 * kWarps, 0, 1, k3g_stream(stream),
+                                          (const unsigned char*)cache + layer_off, (const int*)block_table, page_stride, pages, (const int*)lens, (__nv_bfloat16*)out, n);
+  if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   return k3g_launch_status();
 }

@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const float* 
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.x / ranks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  k3g::follow_launch();
 
   // every warp decides for itself which drafts stay
   bool valid = false, keep = false;
@@ -243,18 +244,10 @@ K3G_API int k3g_verify_draft(const void* target, long long target_stride, const 
   while (ranks > 1 && ((long long)B * ranks > 592 || V < ranks * 2048)) ranks /= 2;
   const int per = kSegs * 4 * ranks;
   const int slice = (int)(((long long)V + per - 1) / per) * kSegs * 4;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(B * ranks), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.stream = k3g_stream(stream);
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)ranks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-  cfg.attrs = at; cfg.numAttrs = 1;
   const bool vec = target_stride % 4 == 0 && (!draft || draft_stride % 4 == 0);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, vec ? verify_draft_kernel<true> : verify_draft_kernel<false>, (const float*)target, target_stride,
-                                           (const float*)draft, draft_stride, (const long long*)ids, (const float*)u, (int*)accepted,
-                                           (long long*)tokens, S, V, slice);
+  const cudaError_t e = k3g_launch_behind(vec ? verify_draft_kernel<true> : verify_draft_kernel<false>, (unsigned)(B * ranks), kThreads, 0, (unsigned)ranks,
+                                          k3g_stream(stream), (const float*)target, target_stride, (const float*)draft, draft_stride, (const long long*)ids,
+                                          (const float*)u, (int*)accepted, (long long*)tokens, S, V, slice);
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   return k3g_launch_status();
 }

@@ -17,6 +17,9 @@ __device__ __forceinline__ void follow_launch() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
+// Loads that stay behind it (the compiler may move read-only ones); the second sees past L1.
+__device__ __forceinline__ int ld_ordered(const int* p) { int v; asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory"); return v; }
+__device__ __forceinline__ int ld_l2(const int* p) { int v; asm volatile("ld.relaxed.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory"); return v; }
 
 struct V8 { unsigned w[4]; };   // eight bf16 = one 16-byte vector
 

@@ -23,13 +23,14 @@
 // 340 (below).  O is made in four products of 128 columns: a pair of chunks is refilled as soon as its quarter of P V is done.
 // The queries' rope columns lie in tensor memory, which makes room for P.
 //
-// What bounds it.  With few rows the cache's bytes, but only where the lengths hide the 20 us that a call's start, end and join take; with many rows, by the formulas,
-// the tensor cores (640 flops a byte for 64 rows).  What a pair waits for in fact is shared memory: a 64 x 128 x 16 step reads 6 KB of it, which is the 48
-// cycles, and with the loaders' stores (147 KB), their loads (84 KB at 64 bytes a clock) and P a pair needs 5900 cycles of it; it takes 7000.
-// More loader warps gain nothing for that reason (16 instead of 8: 351 us).
-// Measured: 8 x 96 rows against 131072 MXFP8 tokens 340 us (630 TFLOP/s, 38% of a dense bf16 product), 48 x 4 x 24 rows against 16384 and their own
-// 512 272 us, 32 x 24 rows against 8229 and 1024 49 us, 64 x 12 rows against their own 4096 49 us (1.8 TB/s), 16 x 2 x 48 rows against bf16
-// pages 57 us, one sequence of 500 tokens 16.5 us.
+// What bounds it.  By the formulas the cache's bytes with few rows, the tensor cores with many (640 flops a byte for 64 rows).  What a pair
+// waits for in fact is shared memory: a 64 x 128 x 16 step reads 6 KB of it, which is the 48 cycles, and with the loaders' stores (147 KB),
+// their loads (84 KB at 64 bytes a clock) and P a pair needs 5900 cycles of it; it takes 7000.  Hence no gain from more loader warps
+// (16 instead of 8: 351 us), from P V in products of 256 columns, which read less but free the chunks later (349), or from the
+// rope columns' product before the last pair of chunks (341).  A call's start, the parts' way out and the join take 17 us beside the pairs.
+// Measured: 8 x 96 rows against 131072 MXFP8 tokens 338 us (648 TFLOP/s, 39% of a dense bf16 product), 48 x 4 x 24 rows against 16384 and
+// their own 512 265 us, 32 x 24 rows against 8229 and 1024 46 us, 64 x 12 rows against their own 4096 45 us (1.9 TB/s), 16 x 2 x 48 rows
+// against bf16 pages 54 us, one sequence of 500 tokens 13 us.
 //
 // Types.  bf16 pages are multiplied as bf16.  MXFP8 codes become f16, not bf16: one conversion and one product for two codes, a third of what bf16
 // takes (which has no conversion from E4M3), and the loaders' instructions are what a tile waits for.  f16 has the bits (a code has four), but not the
@@ -60,7 +61,7 @@ constexpr int kLeastE = -80, kMostE = 120;                   // exponents of 16 
 constexpr float kLag = 4.f, kTop = 10.f;                     // the long document above 340 us, with a lag of 0 (O rescaled for every new maximum) 359
 constexpr int kPartFloats = kRows * kLatent;                 // a part's outputs; its 64 (maximum, sum) pairs lie in a table of their own
 constexpr int kWaitLimit = 1 << 20, kRing = 4, kReaders = kSoftmax / 32 + 1, kTiles = 2;
-constexpr int kStart = 2;                                     // the drafted tokens above 272 us, with 1 336, with 4 283
+constexpr int kStart = 2;                                     // the drafted tokens above 276 us when it was chosen, with 1 336, with 4 283
 
 struct AttnArgs {
   const __nv_bfloat16* q; long long q_stride;
@@ -80,12 +81,9 @@ struct AttnArgs {
 __device__ __forceinline__ unsigned su(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 
 // ---- lengths and the line of (row tile, token tile) pairs ------------------------------------------------------------------
-__device__ __forceinline__ int prefix_tokens(const AttnArgs& a) {
-  return a.prefix_pages ? max(0, (int)min((long long)__ldg(a.prefix_len), (long long)a.prefix_pages * kPageTokens)) : 0;
-}
-__device__ __forceinline__ int own_tokens(const AttnArgs& a, int b) {
-  return max(0, (int)min((long long)__ldg(a.lens + b), (long long)a.max_pages * kPageTokens));
-}
+__device__ __forceinline__ int tokens_of(int len, int pages) { return max(0, min(len, pages * kPageTokens)); }   // pages: 2^20 at most
+__device__ __forceinline__ int prefix_tokens(const AttnArgs& a) { return a.prefix_pages ? tokens_of(ld_ordered(a.prefix_len), a.prefix_pages) : 0; }
+__device__ __forceinline__ int own_tokens(const AttnArgs& a, int b) { return tokens_of(ld_ordered(a.lens + b), a.max_pages); }
 __device__ __forceinline__ int tiles_of(int tokens) { return (tokens + kTile - 1) / kTile; }
 __device__ __forceinline__ int places_of(int tokens) { return tokens ? tiles_of(tokens) + kStart : 0; }   // on the line
 struct Segment {                     // one CTA's stretch of one row tile
@@ -874,7 +872,8 @@ __global__ void __launch_bounds__(128 * GROUPS) latent_attn_join_kernel(const __
   const int row = blockIdx.x * 4 + ((lane >> 1) & 3);
   const bool there = row < rows;
   const int per_seq = a.S * a.heads, b = there ? row / per_seq : 0, in_seq = row - b * per_seq;
-  const int len = __ldg(a.lens + b), ptok = prefix_tokens(a), own = own_tokens(a, b);
+  // read before the wait: the attention kernel lets this one begin when what came before it has ended; from L2, which has what that wrote
+  const int len = ld_l2(a.lens + b), ptok = a.prefix_pages ? tokens_of(ld_l2(a.prefix_len), a.prefix_pages) : 0, own = tokens_of(len, a.max_pages);
   const bool live = there && len >= 0;
   // the parts: those of the row's tile against the prefix, then those against its own tokens; part (CTA, tile) has index CTA + tile
   const int ptile = row / kRows, otile = a.prefix_tiles + b * a.seq_tiles + in_seq / kRows;

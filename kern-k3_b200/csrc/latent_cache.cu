@@ -9,7 +9,8 @@
 // two neighbouring lanes (its maximum is one shuffle), codes move as one 16-byte access per lane, and lanes 0..7 move the
 // rope columns.  No shared memory, no block barrier.  One row and no loop: 131072 rows are stored in 39 us (6.1 TB/s, 93% of a
 // copy), with a loop over rows 44, with two or four rows loaded ahead 40 and 41; 65500 rows are read back in 22.5 us (5.3 TB/s:
-// nearly twice as many bytes are written as read), with two rows ahead 24.8.  A few hundred rows take the launch, 5 us.
+// nearly twice as many bytes are written as read), with two rows ahead 24.8.  Launched behind what comes before, 37.5 and 20.4 us.  A few
+// hundred rows take the launch, 5 us.
 #include "latent_page.cuh"
 #include "k3g_host.h"
 
@@ -52,7 +53,7 @@ __global__ void __launch_bounds__(32 * kWarps) latent_mx8_gather_kernel(const un
                                                                         __nv_bfloat16* __restrict__ out, int n) {
   const int lane = threadIdx.x & 31;
   follow_launch();
-  const int len = lens[0];
+  const int len = ld_ordered(lens);
   const long long t = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (t >= n) return;
   V8 a = {{0u, 0u, 0u, 0u}}, b = a, r = a;

@@ -944,7 +944,7 @@ Space space_of(int B, int S, int heads) {
   s.spans = up(kMaxCtas * 4);
   s.sums = s.spans + up(tiles * 8);
   s.parts = s.sums + up(parts * kRows * 8);
-  s.bytes = s.parts + parts * kPartFloats * 4;
+  s.bytes = s.parts + parts * kPartFloats * 4 + 16;          // parts are stored 32 bytes at a time: the space begins at such a border
   return s;
 }
 
@@ -987,7 +987,7 @@ K3G_API int k3g_latent_attn(const void* q, long long q_stride, const void* cache
   auto kernel = cache_mx8 ? latent_attn_kernel<true> : latent_attn_kernel<false>;
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
-  unsigned char* ws = (unsigned char*)workspace;
+  unsigned char* ws = (unsigned char*)((reinterpret_cast<uintptr_t>(workspace) + 31) & ~(uintptr_t)31);
   const long long rows = (long long)B * S * heads;
   const int ctas = sms < kMaxCtas ? sms : kMaxCtas;
   AttnArgs a = {(const __nv_bfloat16*)q, q_stride, (const unsigned char*)cache + layer_off * unit, page_stride * unit, pages,

@@ -377,6 +377,21 @@ def test_attn_captured_once_serves_growing_lengths(k3g, dev):
         c.compare(bf16_bits(c.out))
 
 
+def test_attn_workspace_at_any_16_bytes(k3g, dev):
+    """Only 16-byte aligned, and exactly as large as asked for: what lies around it stays."""
+    import torch
+    c = Case(dev, 3, 2, 24, 700, [5, 70, 3], seed=32).upload(k3g)
+    n = c.ws.numel()
+    buf = torch.full((n + 64,), 0xA5, dtype=torch.uint8, device=dev)
+    for off in (0, 16, 32, 48):
+        buf.fill_(0xA5)
+        c.out.copy_(to_dev_bf16(c.out0, dev))
+        c.call(k3g, ws=buf[off:off + n])
+        torch.cuda.synchronize()
+        c.compare(bf16_bits(c.out))
+        assert (buf[:off] == 0xA5).all() and (buf[off + n:] == 0xA5).all()
+
+
 def test_attn_workspace_of_a_larger_batch_serves_a_smaller_one(k3g, dev):
     import torch
     big = k3g.latent_attn_workspace(8, 4, 96)

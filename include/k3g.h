@@ -417,6 +417,8 @@ int k3g_latent_mx8_gather(const void* cache, const void* block_table, long long 
  *   - a row that sees no token is zero.  One that sees a NaN, or a score of +infinity, is NaN; a token whose score is -infinity
  *     weighs nothing, but among the tokens that not all steps see (and those in one tile with them) an infinite value makes the
  *     rows that see it NaN.  Rows that do not see it are not touched by it, and what lies behind a page's last token is not used.
+ *   - MXFP8 pages: an element below 2^-33 of the largest in the 16 tokens around it may count as 0, and so may a token's share in
+ *     the outputs (not in the sum of the weights) where it is below 2^-33 of the largest token's.
  *   - prefix_pages = 0 / max_pages = 0: no prefix / no own tokens (the tables, and prefix_len, may be null).
  *   - workspace: 16-byte aligned device memory of k3g_latent_attn_workspace bytes (else K3G_EWORKSPACE), used by one call at a time:
  *     calls that may overlap, and captured graphs that may run together, need one each.  Its content need not be kept.

@@ -101,7 +101,7 @@ struct Tile {                        // where a tile's pages are
 
 // ---- barriers and tensor memory -----------------------------------------------------------------------------------------------
 struct Control {
-  unsigned long long full[5], empty[4], s_full, s_read, p_full, q_full, o_free;
+  unsigned long long full[5], empty[4], q_full[4], s_full, s_read, p_full, o_free;
   unsigned long long ring_full[kRing], ring_empty[kRing], tile_full[kTiles], tile_empty[kTiles];
   Tile tile[kTiles];
   Segment ring[kRing];
@@ -433,10 +433,10 @@ __device__ void issue_tiles(Control& k, unsigned q, unsigned p, unsigned slots) 
   for (unsigned n = 0;; ++n) {
     const Segment s = segment(k, n, true);
     if (s.t1 == 0) return;
-    wait(k, k.q_full, n & 1);
     for (int t = s.t0; t < s.t1; ++t, ++i) {
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {                          // rolled, as everything that runs once a tile: unrolled code is waited for
+        if (t == s.t0) wait(k, k.q_full[c], n & 1);          // the queries come by pairs of chunks, too
         wait(k, k.full[c], i & 1);
         fence_after();
 #pragma unroll
@@ -474,14 +474,15 @@ __device__ __forceinline__ const __nv_bfloat16* query(const AttnArgs& a, const S
 }
 // A segment's queries.  Four threads to a row bring its latent columns into shared memory, zeros where the tile has no row: for bf16 pages
 // copied, for MXFP8 pages made f16, the row's largest element brought to 2^14 .. 2^15.  The rope columns go into tensor memory,
-// 32 of a row from each thread (each row on both halves of the lanes).
+// 32 of a row from each thread (each row on both halves of the lanes).  They are handed over by pairs of chunks, the rope columns with the first.
 template <bool MX8>
 __device__ __forceinline__ void fetch_q(const AttnArgs& a, Control& k, const Segment& s, unsigned n, unsigned q, unsigned rope_at, int tid) {
   const int r = tid >> 2;
   const __nv_bfloat16* src = query(a, s, r);
   const uint4* from = reinterpret_cast<const uint4*>(src) + (tid & 3);
+  const __nv_bfloat16* rope_src = query(a, s, tid & 63);
   uint4 x[16];
-  unsigned top = 0;
+  unsigned top = 0, rope[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     if (MX8) {
@@ -489,46 +490,50 @@ __device__ __forceinline__ void fetch_q(const AttnArgs& a, Control& k, const Seg
     } else {
       const int unit = 4 * i + (tid & 3);
       copy16(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7), reinterpret_cast<const unsigned char*>(src ? from + 4 * i : reinterpret_cast<const uint4*>(a.q)), src != nullptr);
+      if (i % 4 == 3) copies_commit();
     }
   }
-  if (MX8) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, absmax8(V8{{x[i].x, x[i].y, x[i].z, x[i].w}}));
-  }
-  if (MX8) {
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = (int)(top >> 7);                           // exponent field of the largest element; 0: a row of zeros (or of subnormals), 255: not finite
-    const int shift = e == 0 || e == 255 ? 0 : max(e - 127 - 14, -120);   // q' = q * 2^-shift
-    const float up = __uint_as_float((unsigned)(127 - shift) << 23);
-    if ((tid & 3) == 0) k.row_shift[n & 1][r] = (signed char)shift;
-    auto half = [&](unsigned w) {
-      const __half2 h = __floats2half2_rn(bf_lo(w) * up, bf_hi(w) * up);
-      return *reinterpret_cast<const unsigned*>(&h);
-    };
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int unit = 4 * i + (tid & 3);
-      store16(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7), make_uint4(half(x[i].x), half(x[i].y), half(x[i].z), half(x[i].w)));
-    }
-  }
-  const __nv_bfloat16* rope_src = query(a, s, tid & 63);
-  unsigned rope[16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint4 y = rope_src ? __ldg(reinterpret_cast<const uint4*>(rope_src + kLatent + (tid >> 7) * 32) + i) : make_uint4(0u, 0u, 0u, 0u);
     rope[4 * i] = y.x; rope[4 * i + 1] = y.y; rope[4 * i + 2] = y.z; rope[4 * i + 3] = y.w;
   }
+  float up = 1.f;
+  if (MX8) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, absmax8(V8{{x[i].x, x[i].y, x[i].z, x[i].w}}));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = (int)(top >> 7);                           // exponent field of the largest element; 0: a row of zeros (or of subnormals), 255: not finite
+    const int shift = e == 0 || e == 255 ? 0 : max(e - 127 - 14, -120);   // q' = q * 2^-shift
+    up = __uint_as_float((unsigned)(127 - shift) << 23);
+    if ((tid & 3) == 0) k.row_shift[n & 1][r] = (signed char)shift;
+  }
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
                :: K3G_I8(rope, 0), K3G_I8(rope, 8), "r"(rope_at + (tid >> 7) * 16) : "memory");
   tmem_wait_st();
-  if (!MX8) {
-    copies_commit();
-    copies_left<0>();
-  }
-  fence_async();
   fence_before();
-  arrive(k.q_full);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (MX8) {
+      auto half = [&](unsigned w) {
+        const __half2 h = __floats2half2_rn(bf_lo(w) * up, bf_hi(w) * up);
+        return *reinterpret_cast<const unsigned*>(&h);
+      };
+#pragma unroll
+      for (int i = 4 * c; i < 4 * c + 4; ++i) {
+        const int unit = 4 * i + (tid & 3);
+        store16(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7), make_uint4(half(x[i].x), half(x[i].y), half(x[i].z), half(x[i].w)));
+      }
+    } else {
+      if (c == 0) copies_left<3>();
+      if (c == 1) copies_left<2>();
+      if (c == 2) copies_left<1>();
+      if (c == 3) copies_left<0>();
+    }
+    fence_async();
+    arrive(k.q_full[c]);
+  }
 }
 // The four warps that share 32 rows.
 __device__ __forceinline__ void softmax_barrier(int rows) {
@@ -543,13 +548,13 @@ __device__ __forceinline__ bool softmax_vote(int rows, bool mine) {   // the sam
 }
 __device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 
-// Warp w: rows 32 (w % 2) .. of the tile, of page w / 2 % 2 of each token tile 32 tokens (32 (w / 4) ..), of O the columns on the same lanes of two
-// accumulators.
+// Warp w: rows 32 (w % 2) .. of the tile, of page w / 2 % 2 of each token tile 32 tokens (32 (w / 4) ..), of O the columns on the same lanes, 32 of each
+// accumulator.
 template <bool MX8>
 __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigned p_mem, int tid) {
   const int r = tid & 63, half = (tid >> 6) & 1, part = tid >> 7, rows32 = (tid >> 5) & 1, first = half * 64 + part * 32;
   const unsigned lanes = (unsigned)((tid >> 5) & 3) << 21;   // this warp's 32 lanes of tensor memory
-  const unsigned tmem = *(volatile unsigned*)&k.tmem + lanes, o = tmem + part * 128, sc = tmem + kTmemS + part * 32, tq = tmem + kTmemQ;
+  const unsigned tmem = *(volatile unsigned*)&k.tmem + lanes, o = tmem + part * 32, sc = tmem + kTmemS + part * 32, tq = tmem + kTmemQ;
   {
     const Segment s = segment(k, 0, false);
     if (s.t1 == 0) return;
@@ -618,7 +623,7 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigne
           l *= f;
           m = best;
 #pragma unroll 1
-          for (int c = 0; c < 128; c += 32) {
+          for (int c = 0; c < 256; c += 64) {
             unsigned v[32];
             tmem_ld32(o + c, v);
             tmem_wait_ld();
@@ -665,25 +670,25 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigne
     // the last product with this segment's queries is done: the next segment's take their place while P V goes on
     const Segment next = segment(k, n + 1, false);
     if (next.t1 > 0) fetch_q<MX8>(a, k, next, n + 1, q, tq, tid);
-    // this stretch's unnormalised outputs, maximum and sum
-    wait(k, k.empty[3], (i - 1) & 1);
-    fence_after();
+    // this stretch's unnormalised outputs, maximum and sum; the outputs by 128 columns, as P V leaves them
     const bool live_row = query(a, s, r) != nullptr;
     const long long at = (long long)blockIdx.x + s.tile;
     k.best[2 * part + half][r] = l;
     softmax_barrier(rows32);
     if (half + part == 0 && live_row) a.sums[at * kRows + r] = make_float2(m, (k.best[0][r] + k.best[1][r]) + (k.best[2][r] + k.best[3][r]));
     softmax_barrier(rows32);                                 // the sums are read before a maximum takes their place
-    float* dst = a.parts + at * kPartFloats + ((part * 32 + half * 8) * kRows + r) * 8;
+    float* dst = a.parts + at * kPartFloats + ((half * 8 + part * 4) * kRows + r) * 8;
 #pragma unroll 1
-    for (int c = 0; c < 128; c += 32) {
+    for (int u = 0; u < 4; ++u) {
+      wait(k, k.empty[u], (i - 1) & 1);
+      fence_after();
       unsigned v[32];
-      tmem_ld32(o + c, v);
+      tmem_ld32(o + u * 64, v);
       tmem_wait_ld();
       if (live_row) {
 #pragma unroll
         for (int j = 0; j < 32; j += 8)
-          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(dst + ((c >> 6) * 16 + ((c & 63) + j) / 8) * (kRows * 8)), K3G_I8(v, j) : "memory");
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(dst + (u * 16 + j / 8) * (kRows * 8)), K3G_I8(v, j) : "memory");
       }
     }
     fence_before();
@@ -778,13 +783,13 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
     auto init = [](unsigned long long& bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(su(&bar)), "r"(n)); };
     for (int u = 0; u < 5; ++u) init(k.full[u], kLoaders / 32);
 #pragma unroll 1
-    for (int u = 0; u < 4; ++u) init(k.empty[u], 1);
+    for (int u = 0; u < 4; ++u) { init(k.empty[u], 1); init(k.q_full[u], kSoftmax); }
     init(k.s_full, 1); init(k.s_read, kSoftmax / 32); init(k.p_full, kSoftmax);
 #pragma unroll 1
     for (int u = 0; u < kRing; ++u) { init(k.ring_full[u], 1); init(k.ring_empty[u], kReaders); }
 #pragma unroll 1
     for (int u = 0; u < kTiles; ++u) { init(k.tile_full[u], 1); init(k.tile_empty[u], kLoaders / 32); }
-    init(k.q_full, kSoftmax); init(k.o_free, kSoftmax);
+    init(k.o_free, kSoftmax);
     k.abort = 0;
 #pragma unroll 1
     for (int i = 0; i < 8; ++i) k.poison[i >> 2][i & 3] = 0;

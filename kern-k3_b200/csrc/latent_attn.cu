@@ -184,8 +184,9 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // ---- loaders ----------------------------------------------------------------------------------------------------------------------
-// Warp w looks after tokens 16 w .. + 15 of a tile, lane x after tokens 16 w + x % 8 and + 8 and of each pair of chunks the 32 columns x / 8: one scale
-// block.  Eight lanes that store together write the same columns of eight tokens, which the swizzle spreads over all banks.
+// Warp w looks after tokens 16 w .. + 15 of a tile, a lane after two of them, 8 apart, and of each pair of chunks after 32 columns: one scale
+// block.  Eight lanes that load together read 64 bytes of four tokens each, and store to all banks: two units of four tokens, swizzled.  (32 bytes
+// of eight tokens: 336 us for the long document above instead of 321; 128 bytes of two, for which half of the lanes turn their words round: 320.)
 __device__ __forceinline__ unsigned clean(unsigned w, unsigned top, unsigned& bad) {   // a pair of 16-bit floats with NaN and infinities taken out
   if ((w & top) == top) { w &= 0xffff0000u; bad = 1; }
   if ((w & (top << 16)) == (top << 16)) { w &= 0x0000ffffu; bad = 1; }
@@ -248,7 +249,7 @@ struct Loader {
     bool careful, live;
   } here, next;
   __device__ __forceinline__ Loader(const AttnArgs& a, Control& k, unsigned slots, int t) : a(a), k(k), slots(slots), tid(t), lane(t & 31),
-      token((t >> 5) * 16 + (t & 7)), block(lane >> 3) {
+      token((t >> 5) * 16 + ((t >> 1) & 7)), block((t & 1) + 2 * (lane >> 4)) {
 #pragma unroll
     for (int x = 0; x < 4; ++x) put_at[x] = slots + (block >> 1) * kChunk + unit_at(token, (block & 1) * 4 + x);
   }

@@ -19,18 +19,19 @@
 //   8 softmax warps  S from tensor memory, running maximum, P = 2^(S - m) rounded to 16 bits into shared memory; O scaled, read and written out.
 // Why M = 64: a 128-row O of 512 columns fills the whole tensor memory and leaves no room for S.  The weight-stationary form puts
 // a 64-row tile on all 128 lanes and reaches 48 cycles per 64 x 128 x 16 step, the plain form 64 (measured; 32 would be full rate).
-// Why 128 tokens: a 64 x 64 x 16 step costs 44 cycles.  Tiles of one page in two buffers, which let all roles work at once, took 425 us where this takes
-// 340 (below).  O is made in four products of 128 columns: a pair of chunks is refilled as soon as its quarter of P V is done.
+// Why 128 tokens: a 64 x 64 x 16 step costs 44 cycles.  Tiles of one page in two buffers, which let all roles work at once, took 425 us where this took
+// 340.  O is made in four products of 128 columns: a pair of chunks is refilled as soon as its quarter of P V is done.
 // The queries' rope columns lie in tensor memory, which makes room for P.
 //
 // What bounds it.  By the formulas the cache's bytes with few rows, the tensor cores with many (640 flops a byte for 64 rows).  What a pair
 // waits for in fact is shared memory: a 64 x 128 x 16 step reads 6 KB of it, which is the 48 cycles, and with the loaders' stores (147 KB),
-// their loads (84 KB at 64 bytes a clock) and P a pair needs 5900 cycles of it; it takes 7000.  Hence no gain from more loader warps
-// (16 instead of 8: 351 us), from P V in products of 256 columns, which read less but free the chunks later (349), or from the
-// rope columns' product before the last pair of chunks (341).  A call's start, the parts' way out and the join take 17 us beside the pairs.
-// Measured: 8 x 96 rows against 131072 MXFP8 tokens 338 us (648 TFLOP/s, 39% of a dense bf16 product), 48 x 4 x 24 rows against 16384 and
-// their own 512 265 us, 32 x 24 rows against 8229 and 1024 46 us, 64 x 12 rows against their own 4096 45 us (1.9 TB/s), 16 x 2 x 48 rows
-// against bf16 pages 54 us, one sequence of 500 tokens 13 us.
+// their loads (84 KB, 16 wavefronts for 1 KB) and P a pair needs 6700 cycles of it (counted: tensor cores 3400, load and store pipe 3300); it takes 7000.
+// Hence no gain from more loader warps (16 instead of 8: 346 us instead of 321), from P V in products of 256 columns, which read less but
+// free the chunks later (349 instead of 339), from one accumulator for latent and rope columns (323), or from the rope columns' product before the last pair
+// of chunks (341 instead of 340).  A call's start, the parts' way out and the join take 17 us beside the pairs.
+// Measured: 8 x 96 rows against 131072 MXFP8 tokens 321 us (333 when other inputs come every time: 659 TFLOP/s, 40% of a dense bf16 product),
+// 48 x 4 x 24 rows against 16384 and their own 512 258 us, 32 x 24 rows against 8229 and 1024 45 us, 64 x 12 rows against their own 4096
+// 43 us (2.0 TB/s), 16 x 2 x 48 rows against bf16 pages 53 us, one sequence of 500 tokens 12.4 us.
 //
 // Types.  bf16 pages are multiplied as bf16.  MXFP8 codes become f16, not bf16: one conversion and one product for two codes, a third of what bf16
 // takes (which has no conversion from E4M3), and the loaders' instructions are what a tile waits for.  f16 has the bits (a code has four), but not the
@@ -58,7 +59,7 @@ constexpr int kSmemQ = 8 * kQChunk, kSmemP = 2 * kQChunk, kSmemK = 9 * kChunk, k
 // half), the rope columns' part of S 320..383 (MXFP8), the queries' rope columns 384..415 (the same on both halves)
 constexpr int kTmemS = 256, kTmemR = 320, kTmemQ = 384;
 constexpr int kLeastE = -80, kMostE = 120;                   // exponents of 16 tokens: sums of 2^-E stay in range
-constexpr float kLag = 4.f, kTop = 10.f;                     // the long document above 340 us, with a lag of 0 (O rescaled for every new maximum) 359
+constexpr float kLag = 4.f, kTop = 10.f;                     // the long document above 340 us when it was chosen, with a lag of 0 (O rescaled for every new maximum) 359
 constexpr int kPartFloats = kRows * kLatent;                 // a part's outputs; its 64 (maximum, sum) pairs lie in a table of their own
 constexpr int kWaitLimit = 1 << 20, kRing = 4, kReaders = kSoftmax / 32 + 1, kTiles = 2;
 constexpr int kStart = 2;                                     // the drafted tokens above 276 us when it was chosen, with 1 336, with 4 283
@@ -768,7 +769,7 @@ __device__ void plan(const AttnArgs& a, Control& k, int ptok, int page_bytes, in
       // steps of a sequence do not see all of its last S - 1 tokens: a value that is not finite must not reach the others through 0 * NaN
       w.careful = s.b >= 0 && a.S > 1 && (t + 1) * kTile > s.tokens - (a.S - 1);
       plan_tile(k, i, w, lane);
-      // L2 has the pages before the loaders ask for them (two or three tiles ahead: 340 us for the long document, without it 346)
+      // L2 has the pages before the loaders ask for them (two or three tiles ahead: 340 us for the long document when it was added, without it 346)
       if (lane < 2 && (lane ? w.tokens[1] : w.tokens[0])) prefetch(lane ? w.page[1] : w.page[0], page_bytes);
     }
   }

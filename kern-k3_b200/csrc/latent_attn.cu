@@ -23,12 +23,13 @@
 // 340.  O is made in four products of 128 columns: a pair of chunks is refilled as soon as its quarter of P V is done.
 // The queries' rope columns lie in tensor memory, which makes room for P.
 //
-// What bounds it.  By the formulas the cache's bytes with few rows, the tensor cores with many (640 flops a byte for 64 rows).  What a pair
-// waits for in fact is shared memory: a 64 x 128 x 16 step reads 6 KB of it, which is the 48 cycles, and with the loaders' stores (147 KB),
-// their loads (84 KB, 16 wavefronts for 1 KB) and P a pair needs 6700 cycles of it (counted: tensor cores 3400, load and store pipe 3300); it takes 7000.
-// Hence no gain from more loader warps (16 instead of 8: 346 us instead of 321), from P V in products of 256 columns, which read less but
-// free the chunks later (349 instead of 339), from one accumulator for latent and rope columns (323), or from the rope columns' product before the last pair
-// of chunks (341 instead of 340).  A call's start, the parts' way out and the join take 17 us beside the pairs.
+// What bounds it.  By the formulas the cache's bytes with few rows, the tensor cores with many (640 flops a byte for 64 rows).  A pair takes
+// 7000 cycles, in two phases that one buffer of 128 tokens keeps apart.  From P to S, 4600: the products, 3400 cycles in which a 64 x 128 x 16
+// step reads 6 KB of shared memory, which is its 48 cycles, and the loaders' stores between them, 1300 wavefronts.  From S to P, 2400: S out
+// of tensor memory, maximum, vote, exponentials.  Hence no gain from more loader warps (16 instead of 8: 346 us instead of 321), from P V in products
+// of 256 columns, which read less but free the chunks later (349 instead of 339), from one accumulator for latent and rope columns (323
+// instead of 321), or from the rope columns' product before the last pair of chunks (341 instead of 340).  A call's start, the parts' way out and the
+// join take 17 us beside the pairs.
 // Measured: 8 x 96 rows against 131072 MXFP8 tokens 321 us (333 when other inputs come every time: 659 TFLOP/s, 40% of a dense bf16 product),
 // 48 x 4 x 24 rows against 16384 and their own 512 258 us, 32 x 24 rows against 8229 and 1024 45 us, 64 x 12 rows against their own 4096
 // 43 us (2.0 TB/s), 16 x 2 x 48 rows against bf16 pages 53 us, one sequence of 500 tokens 12.4 us.

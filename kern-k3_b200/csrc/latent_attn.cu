@@ -135,6 +135,12 @@ __device__ __forceinline__ void wait(Control& k, unsigned long long& bar, unsign
   }
   *(volatile int*)&k.abort = 1;
 }
+// The first poll of a wait, for a warp that has something to do until it needs the answer.
+__device__ __forceinline__ unsigned poll(unsigned long long& bar, unsigned parity) {
+  unsigned ok;
+  asm volatile("{.reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}" : "=r"(ok) : "r"(su(&bar)), "r"(parity) : "memory");
+  return ok;
+}
 __device__ __forceinline__ void arrive(unsigned long long& bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(su(&bar)) : "memory"); }
 __device__ __forceinline__ void commit(unsigned lead, unsigned long long& bar) {
   asm volatile("{.reg .pred e; setp.ne.b32 e, %1, 0; @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];}" :: "r"(su(&bar)), "r"(lead) : "memory");
@@ -374,17 +380,20 @@ struct Loader {
     hand_over(0);
     copy(8);
     copies_commit();
+    const unsigned e1 = poll(k.empty[1], (i - 1) & 1);
     const Units u1 = convert(1, most);
-    empty(i, 1);
+    if (!e1) empty(i, 1);
     put(1, u1);
     hand_over(1);
     if (MX8) {
+      const unsigned e2 = poll(k.empty[2], (i - 1) & 1);
       const Units u2 = convert(2, most);
-      empty(i, 2);
+      if (!e2) empty(i, 2);
       put(2, u2);
       hand_over(2);
+      const unsigned e3 = poll(k.empty[3], (i - 1) & 1);
       const Units u3 = convert(3, most);
-      empty(i, 3);
+      if (!e3) empty(i, 3);
       put(3, u3);
       hand_over(3);
       next = where(i + 1);

@@ -316,39 +316,32 @@ struct Loader {
       if (bad) atomicOr(&k.poison[i & 1][at >> 5], 1u << (at & 31));
     }
   }
-  struct Units { uint4 u[2][4]; };
-  __device__ __forceinline__ Units convert(int p, unsigned most) {   // of pair p (bf16: 0 or 1)
+  struct Units { uint4 u[4]; };
+  __device__ __forceinline__ Units convert(int p, int g, unsigned most) {   // token g of pair p (bf16: 0 or 1)
     Units o;
+    if (MX8) {
+      const unsigned s = f16_scale(most, (scales[g].w[p] >> (block * 8)) & 0xffu);
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      if (MX8) {
-        const unsigned s = f16_scale(most, (scales[g].w[p] >> (block * 8)) & 0xffu);
+      for (int x = 0; x < 4; ++x) {
+        mx8_to_f16x4(code[p][g].w[2 * x], s, o.u[x].x, o.u[x].y);
+        mx8_to_f16x4(code[p][g].w[2 * x + 1], s, o.u[x].z, o.u[x].w);
+      }
+    } else {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          mx8_to_f16x4(code[p][g].w[2 * x], s, o.u[g][x].x, o.u[g][x].y);
-          mx8_to_f16x4(code[p][g].w[2 * x + 1], s, o.u[g][x].z, o.u[g][x].w);
-        }
-      } else {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const V16& v = code[(2 * p + (x >> 1)) & 3][g];
-          o.u[g][x] = make_uint4(v.w[4 * (x & 1)], v.w[4 * (x & 1) + 1], v.w[4 * (x & 1) + 2], v.w[4 * (x & 1) + 3]);
-        }
+      for (int x = 0; x < 4; ++x) {
+        const V16& v = code[(2 * p + (x >> 1)) & 3][g];
+        o.u[x] = make_uint4(v.w[4 * (x & 1)], v.w[4 * (x & 1) + 1], v.w[4 * (x & 1) + 2], v.w[4 * (x & 1) + 3]);
       }
     }
-    if (here.tokens < kPageTokens) {
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if ((token & 63) + 8 * g >= here.tokens) o.u[g][0] = o.u[g][1] = o.u[g][2] = o.u[g][3] = make_uint4(0u, 0u, 0u, 0u);
-    }
+    if ((token & 63) + 8 * g >= here.tokens) o.u[0] = o.u[1] = o.u[2] = o.u[3] = make_uint4(0u, 0u, 0u, 0u);
     return o;
   }
   unsigned bad[2];                                           // the thread's tokens have values that are not finite
-  __device__ __forceinline__ void put(int p, const Units& o) {
+  __device__ __forceinline__ void put(int p, int g, const Units& o) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) store16(put_at[x] + 2 * p * kChunk + g * 1024, o.u[g][x]);
+    for (int x = 0; x < 4; ++x) store16(put_at[x] + 2 * p * kChunk + g * 1024, o.u[x]);
+  }
+  __device__ __forceinline__ void clean_put(int p) {
     if (here.careful) {
       clean_units(slots + (2 * p + (block >> 1)) * kChunk, token, (block & 1) * 4, 4, MX8 ? 0x7c00u : 0x7f80u, bad[0]);
       clean_units(slots + (2 * p + (block >> 1)) * kChunk, token + 8, (block & 1) * 4, 4, MX8 ? 0x7c00u : 0x7f80u, bad[1]);
@@ -371,33 +364,47 @@ struct Loader {
       }
       most = min(max(__reduce_max_sync(0xffffffffu, most), (unsigned)(128 + kLeastE)), (unsigned)(128 + kMostE)) - 1;
     }
-    const Units u0 = convert(0, most);
+    Units u = convert(0, 0, most), v = convert(0, 1, most);
     empty(i, 0);
     if (tid < 4) k.poison[(i + 1) & 1][tid] = 0;             // the tile before this one has been read, the next is not there yet
     if (MX8 && lane == 0) k.exponent[tid >> 5] = (int)most - 127;   // E
     if ((tid & 127) == 0) k.tokens[tid >> 7] = here.tokens;
-    put(0, u0);
+    put(0, 0, u);
+    const unsigned e1 = poll(k.empty[1], (i - 1) & 1);
+    u = convert(1, 0, most);                                 // while the stores before it go out
+    put(0, 1, v);
+    v = convert(1, 1, most);
+    clean_put(0);
     hand_over(0);
     copy(8);
     copies_commit();
-    const unsigned e1 = poll(k.empty[1], (i - 1) & 1);
-    const Units u1 = convert(1, most);
     if (!e1) empty(i, 1);
-    put(1, u1);
-    hand_over(1);
+    put(1, 0, u);
     if (MX8) {
       const unsigned e2 = poll(k.empty[2], (i - 1) & 1);
-      const Units u2 = convert(2, most);
+      u = convert(2, 0, most);
+      put(1, 1, v);
+      v = convert(2, 1, most);
+      clean_put(1);
+      hand_over(1);
       if (!e2) empty(i, 2);
-      put(2, u2);
-      hand_over(2);
+      put(2, 0, u);
       const unsigned e3 = poll(k.empty[3], (i - 1) & 1);
-      const Units u3 = convert(3, most);
+      u = convert(3, 0, most);
+      put(2, 1, v);
+      v = convert(3, 1, most);
+      clean_put(2);
+      hand_over(2);
       if (!e3) empty(i, 3);
-      put(3, u3);
+      put(3, 0, u);
+      put(3, 1, v);
+      clean_put(3);
       hand_over(3);
       next = where(i + 1);
     } else {                                                 // the other half of bf16 pages is copied
+      put(1, 1, v);
+      clean_put(1);
+      hand_over(1);
       next = where(i + 1);
       load<0, 4>(next);
       empty(i, 2);

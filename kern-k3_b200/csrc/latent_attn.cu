@@ -373,9 +373,9 @@ struct Loader {
     const unsigned e1 = poll(k.empty[1], (i - 1) & 1);
     u = convert(1, 0, most);                                 // while the stores before it go out
     put(0, 1, v);
-    v = convert(1, 1, most);
     clean_put(0);
     hand_over(0);
+    v = convert(1, 1, most);
     copy(8);
     copies_commit();
     if (!e1) empty(i, 1);
@@ -384,17 +384,17 @@ struct Loader {
       const unsigned e2 = poll(k.empty[2], (i - 1) & 1);
       u = convert(2, 0, most);
       put(1, 1, v);
-      v = convert(2, 1, most);
       clean_put(1);
       hand_over(1);
+      v = convert(2, 1, most);
       if (!e2) empty(i, 2);
       put(2, 0, u);
       const unsigned e3 = poll(k.empty[3], (i - 1) & 1);
       u = convert(3, 0, most);
       put(2, 1, v);
-      v = convert(3, 1, most);
       clean_put(2);
       hand_over(2);
+      v = convert(3, 1, most);
       if (!e3) empty(i, 3);
       put(3, 0, u);
       put(3, 1, v);

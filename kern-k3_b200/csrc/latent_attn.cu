@@ -376,10 +376,10 @@ struct Loader {
     clean_put(0);
     hand_over(0);
     v = convert(1, 1, most);
-    copy(8);
-    copies_commit();
     if (!e1) empty(i, 1);
     put(1, 0, u);
+    copy(8);
+    copies_commit();
     if (MX8) {
       const unsigned e2 = poll(k.empty[2], (i - 1) & 1);
       u = convert(2, 0, most);
@@ -400,7 +400,6 @@ struct Loader {
       put(3, 1, v);
       clean_put(3);
       hand_over(3);
-      next = where(i + 1);
     } else {                                                 // the other half of bf16 pages is copied
       put(1, 1, v);
       clean_put(1);
@@ -428,6 +427,7 @@ struct Loader {
     }
     hand_over(4);
     if (MX8) {
+      next = where(i + 1);
       load<0, 3>(next);
       wait(k, k.s_read, i & 1);
       load<3, 4>(next);

@@ -453,17 +453,20 @@ __device__ void issue_tiles(Control& k, unsigned q, unsigned p, unsigned slots) 
     const Segment s = segment(k, n, true);
     if (s.t1 == 0) return;
     for (int t = s.t0; t < s.t1; ++t, ++i) {
+      unsigned ok = 0;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {                          // rolled, as everything that runs once a tile: unrolled code is waited for
         if (t == s.t0) wait(k, k.q_full[c], n & 1);          // the queries come by pairs of chunks, too
-        wait(k, k.full[c], i & 1);
+        if (!ok) wait(k, k.full[c], i & 1);
         fence_after();
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 8; ++j) {
+          if (j == 6) ok = poll(k.full[c + 1], i & 1);       // asked while the products are issued
           mma_ws(lead, sc, dq + (((2 * c + (j >> 2)) * kQChunk + (j & 3) * 32) >> 4), dk + (((2 * c + (j >> 2)) * kChunk + (j & 3) * 32) >> 4),
                  shape_of(!MX8, 0), c + j > 0);
+        }
       }
-      wait(k, k.full[4], i & 1);
+      if (!ok) wait(k, k.full[4], i & 1);
       fence_after();
 #pragma unroll
       for (int j = 0; j < 4; ++j) mma_ws_tmem(lead, sr, tmem + kTmemQ + j * 8, dk + ((8 * kChunk + j * 32) >> 4), shape_of(true, 0), !MX8 || j > 0);

@@ -24,15 +24,16 @@
 // The queries' rope columns lie in tensor memory, which makes room for P.
 //
 // What bounds it.  By the formulas the cache's bytes with few rows, the tensor cores with many (640 flops a byte for 64 rows).  A pair takes
-// 7000 cycles, in two phases that one buffer of 128 tokens keeps apart.  From P to S, 4600: the products, 3400 cycles in which a 64 x 128 x 16
-// step reads 6 KB of shared memory, which is its 48 cycles, and the loaders' stores between them, 1300 wavefronts.  From S to P, 2400: S out
-// of tensor memory, maximum, vote, exponentials.  Hence no gain from more loader warps (16 instead of 8: 346 us instead of 321), from P V in products
-// of 256 columns, which read less but free the chunks later (349 instead of 339), from one accumulator for latent and rope columns (323
-// instead of 321), or from the rope columns' product before the last pair of chunks (341 instead of 340).  A call's start, the parts' way out and the
-// join take 17 us beside the pairs.
-// Measured: 8 x 96 rows against 131072 MXFP8 tokens 321 us (333 when other inputs come every time: 659 TFLOP/s, 40% of a dense bf16 product),
-// 48 x 4 x 24 rows against 16384 and their own 512 258 us, 32 x 24 rows against 8229 and 1024 45 us, 64 x 12 rows against their own 4096
-// 43 us (2.0 TB/s), 16 x 2 x 48 rows against bf16 pages 53 us, one sequence of 500 tokens 12.4 us.
+// 6300 cycles, in two phases that one buffer of 128 tokens keeps apart.  From P to S, 4400: the products, 3400 cycles in which a 64 x 128 x 16
+// step reads 6 KB of shared memory, which is its 48 cycles, and the loaders' conversions and stores between them.  From S to P, 1900: S out of
+// tensor memory, maximum, vote, exponentials.  What the loaders wait for counts: conversions between the stores, polls ahead of the waits and
+// the next tile's place read last brought 321 us down to 298 (for the long document below).  No gain came from more loader warps (16 instead of 8: 346
+// us instead of 321), from P V in products of 256 columns, which read less but free the chunks later (349 instead of 339), from one
+// accumulator for latent and rope columns (315 instead of 309), or from the rope columns' product before the last pair of chunks (308
+// instead of 303).  A call's start, the parts' way out and the join take 17 us beside the pairs.
+// Measured: 8 x 96 rows against 131072 MXFP8 tokens 298 us (321 in a long run with other inputs every time: 683 TFLOP/s, 41% of a dense bf16
+// product), 48 x 4 x 24 rows against 16384 and their own 512 251 us, 32 x 24 rows against 8229 and 1024 43 us, 64 x 12 rows against
+// their own 4096 41 us (2.1 TB/s), 16 x 2 x 48 rows against bf16 pages 52 us, one sequence of 500 tokens 12.6 us.
 //
 // Types.  bf16 pages are multiplied as bf16.  MXFP8 codes become f16, not bf16: one conversion and one product for two codes, a third of what bf16
 // takes (which has no conversion from E4M3), and the loaders' instructions are what a tile waits for.  f16 has the bits (a code has four), but not the

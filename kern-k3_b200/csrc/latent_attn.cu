@@ -33,7 +33,7 @@
 // instead of 303).  A call's start, the parts' way out and the join take 17 us beside the pairs.
 // Measured: 8 x 96 rows against 131072 MXFP8 tokens 298 us (321 in a long run with other inputs every time: 683 TFLOP/s, 41% of a dense bf16
 // product), 48 x 4 x 24 rows against 16384 and their own 512 251 us, 32 x 24 rows against 8229 and 1024 43 us, 64 x 12 rows against
-// their own 4096 41 us (2.1 TB/s), 16 x 2 x 48 rows against bf16 pages 52 us, one sequence of 500 tokens 12.6 us.
+// their own 4096 41 us (2.1 TB/s), 16 x 2 x 48 rows against bf16 pages 48 us (53 with the next tile asked for before this one was copied), one sequence of 500 tokens 12.6 us.
 //
 // Types.  bf16 pages are multiplied as bf16.  MXFP8 codes become f16, not bf16: one conversion and one product for two codes, a third of what bf16
 // takes (which has no conversion from E4M3), and the loaders' instructions are what a tile waits for.  f16 has the bits (a code has four), but not the
@@ -405,8 +405,6 @@ struct Loader {
       put(1, 1, v);
       clean_put(1);
       hand_over(1);
-      next = where(i + 1);
-      load<0, 4>(next);
       empty(i, 2);
       copy(4); copy(5);
       copies_commit();
@@ -427,11 +425,13 @@ struct Loader {
       if (bad[1]) atomicOr(&k.poison[i & 1][token >> 5], 256u << (token & 31));
     }
     hand_over(4);
+    next = where(i + 1);
     if (MX8) {
-      next = where(i + 1);
       load<0, 3>(next);
       wait(k, k.s_read, i & 1);
       load<3, 4>(next);
+    } else {
+      load<0, 4>(next);
     }
     here = next;
   }

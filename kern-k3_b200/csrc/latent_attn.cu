@@ -696,6 +696,7 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigne
     // this stretch's unnormalised outputs, maximum and sum; the outputs by 128 columns, as P V leaves them
     const bool live_row = query(a, s, r) != nullptr;
     const long long at = (long long)blockIdx.x + s.tile;
+    softmax_barrier(rows32);                                 // the last tile's maxima have been read by all four warps
     k.best[2 * part + half][r] = l;
     softmax_barrier(rows32);
     if (half + part == 0 && live_row) a.sums[at * kRows + r] = make_float2(m, (k.best[0][r] + k.best[1][r]) + (k.best[2][r] + k.best[3][r]));

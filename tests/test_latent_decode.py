@@ -377,6 +377,22 @@ def test_attn_captured_once_serves_growing_lengths(k3g, dev):
         c.compare(bf16_bits(c.out))
 
 
+@pytest.mark.parametrize("mx8", [True, False])
+def test_attn_stretches_of_one_tile_one_after_another(k3g, dev, mx8):
+    """Hundreds of sequences that fit one tile: every CTA takes several stretches of a single tile, in which the exchange of the row maxima is
+    followed at once by that of the sums through the same words.  The oracle's results, and the same bits in thirty runs."""
+    import torch
+    c = Case(dev, 600, 1, 24, 0, [1 + (i * 53) % 128 for i in range(600)], mx8=mx8, seed=33, layers=1).upload(k3g)
+    c.call(k3g)
+    torch.cuda.synchronize()
+    c.compare(bf16_bits(c.out))
+    first = c.out.clone()
+    for _ in range(30):
+        c.out.zero_()
+        c.call(k3g)
+        assert torch.equal(c.out.view(torch.int16), first.view(torch.int16))
+
+
 def test_attn_workspace_at_any_16_bytes(k3g, dev):
     """Only 16-byte aligned, and exactly as large as asked for: what lies around it stays."""
     import torch

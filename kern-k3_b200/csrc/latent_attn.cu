@@ -104,7 +104,7 @@ struct Tile {                        // where a tile's pages are
 
 // ---- barriers and tensor memory -----------------------------------------------------------------------------------------------
 struct Control {
-  unsigned long long full[5], empty[4], q_full[4], s_full, s_read, p_full, o_free;
+  unsigned long long full[5], empty[4], q_full[4], s_full, s_read, p_full, o_free, drained;
   unsigned long long ring_full[kRing], ring_empty[kRing], tile_full[kTiles], tile_empty[kTiles];
   Tile tile[kTiles];
   Segment ring[kRing];
@@ -122,7 +122,8 @@ struct Control {
 };
 
 // Every wait ends: after kWaitLimit polls, or as soon as another wait of the CTA has expired.  The roles then run through what is
-// left without waiting (every access stays where it was), and the call's result is NaN.
+// left without waiting (every access stays where it was: the rings hold end marks before the plan's first entries, and a mixed one of two entries
+// names rows and pages of either), the products on their way are waited for before tensor memory is given back, and the call's result is NaN.
 __device__ __forceinline__ void wait(Control& k, unsigned long long& bar, unsigned parity, unsigned nap = 0) {
   unsigned ok;
   asm volatile("{.reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}" : "=r"(ok) : "r"(su(&bar)), "r"(parity) : "memory");
@@ -452,7 +453,7 @@ __device__ void issue_tiles(Control& k, unsigned q, unsigned p, unsigned slots) 
   unsigned i = 0;
   for (unsigned n = 0;; ++n) {
     const Segment s = segment(k, n, true);
-    if (s.t1 == 0) return;
+    if (s.t1 == 0) break;
     for (int t = s.t0; t < s.t1; ++t, ++i) {
       unsigned ok = 0;
 #pragma unroll 1
@@ -485,6 +486,9 @@ __device__ void issue_tiles(Control& k, unsigned q, unsigned p, unsigned slots) 
       }
     }
   }
+  commit(lead, k.drained);                                   // no product is on its way when the CTA ends, whoever gave up a wait
+#pragma unroll 1
+  for (int x = 0; x < kWaitLimit && !poll(k.drained, 0); ++x) {}
 }
 
 // ---- softmax ----------------------------------------------------------------------------------------------------------------------------
@@ -770,7 +774,7 @@ __device__ void plan(const AttnArgs& a, Control& k, int ptok, int page_bytes, in
     }
     __syncwarp();
     if (s.t1 == 0) {
-      plan_tile(k, i, Tile{{nullptr, nullptr}, {0, 0}, 0, 0}, lane);
+      plan_tile(k, i, Tile{{a.cache, a.cache}, {0, 0}, 0, 0}, lane);
       return;
     }
     const int pages = (s.tokens + kPageTokens - 1) / kPageTokens;
@@ -813,10 +817,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_attn_kernel(const __grid_c
     for (int u = 0; u < kRing; ++u) { init(k.ring_full[u], 1); init(k.ring_empty[u], kReaders); }
 #pragma unroll 1
     for (int u = 0; u < kTiles; ++u) { init(k.tile_full[u], 1); init(k.tile_empty[u], kLoaders / 32); }
-    init(k.o_free, kSoftmax);
+    init(k.o_free, kSoftmax); init(k.drained, 1);
     k.abort = 0;
 #pragma unroll 1
     for (int i = 0; i < 8; ++i) k.poison[i >> 2][i & 3] = 0;
+#pragma unroll 1
+    for (int u = 0; u < kRing; ++u) k.ring[u] = Segment{0, -1, 0, 0, 0, 0};
+#pragma unroll 1
+    for (int u = 0; u < kTiles; ++u) k.tile[u] = Tile{{a.cache, a.cache}, {0, 0}, 0, 0};
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(su(&k.tmem)) : "memory");

@@ -96,3 +96,31 @@ def test_verify_oracle_gives_back_the_target_distribution():
         _, tok = verify_oracle(np.broadcast_to(p, (B, 2, V)), np.broadcast_to(q, (B, 1, V)), np.full((B, 1), x), grid)
         count += q[x] * np.bincount(tok[:, 0], minlength=V) / B
     assert np.allclose(count, p, atol=1e-9)                      # the grid's 24 points divide every boundary evenly
+
+
+def test_warps_shares_of_registers_are_what_the_attention_is_launched_with(tmp_path):
+    """The warps of the attention kernel divide the registers that its block is launched with; a compiler that gave it fewer would leave
+    setmaxnreg.inc waiting for good.  The shares are read from the source, the launch from what ptxas prints."""
+    import os
+    import re
+    import shutil
+    import subprocess
+    import sys
+    nvcc = os.environ.get("NVCC", "nvcc")
+    if not shutil.which(nvcc):
+        pytest.skip("no nvcc")
+    here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "kern-k3_b200")
+    sys.path.insert(0, here)
+    import build
+    source = open(os.path.join(here, "csrc", "latent_attn.cu")).read()
+    softmax, loaders = (int(x) for x in re.findall(r"setmaxnreg\.inc\.sync\.aligned\.u32 (\d+)", source))
+    rest, = (int(x) for x in re.findall(r"setmaxnreg\.dec\.sync\.aligned\.u32 (\d+)", source))
+    sizes = {k: int(v) for k, v in re.findall(r"(kSoftmax|kLoaders) = (\d+)", source)}
+    r = subprocess.run([nvcc] + build.ARCH + build.COMMON + ["-Xptxas", "-v", "-cubin", "-I", os.path.join(here, "..", "include"), os.path.join(here, "csrc", "latent_attn.cu"),
+                                                             "-o", str(tmp_path / "attn.cubin")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    used = [int(n) for n in re.findall(r"Compiling entry function '\S*latent_attn_kernel\S*'.*?Used (\d+) registers", r.stdout + r.stderr, re.S)]
+    assert len(used) == 2
+    threads = sizes["kSoftmax"] + sizes["kLoaders"] + 128
+    for n in used:
+        assert sizes["kSoftmax"] * softmax + sizes["kLoaders"] * loaders + 128 * rest <= threads * ((n + 7) // 8 * 8)

@@ -17,8 +17,18 @@ __device__ __forceinline__ void follow_launch() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
-// Loads that stay behind it (the compiler may move read-only ones); the second sees past L1.
+// Loads of such kernels.  They stay behind the wait and take the coherent path: a launch that another one wrote for has begun while that one
+// was still writing, so nothing it reads is read-only for as long as it runs, which is what ld.global.nc, __ldg and const __restrict__ ask for.
 __device__ __forceinline__ int ld_ordered(const int* p) { int v; asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory"); return v; }
+__device__ __forceinline__ long long ld_ordered(const long long* p) { long long v; asm volatile("ld.global.b64 %0, [%1];" : "=l"(v) : "l"(p) : "memory"); return v; }
+__device__ __forceinline__ float ld_ordered(const float* p) { float v; asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p)); return v; }
+__device__ __forceinline__ float4 ld_ordered(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ unsigned ld_ordered(const unsigned char* p) { unsigned v; asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p)); return v; }
+// The same past L1, for what is read before the wait.
 __device__ __forceinline__ int ld_l2(const int* p) { int v; asm volatile("ld.relaxed.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory"); return v; }
 
 struct V8 { unsigned w[4]; };   // eight bf16 = one 16-byte vector
@@ -28,6 +38,13 @@ struct V8 { unsigned w[4]; };   // eight bf16 = one 16-byte vector
 __device__ __forceinline__ V8 ld_stream(const void* p) {
   V8 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "l"(p));
+  return v;
+}
+// The same on the coherent path, for kernels launched behind others.
+__device__ __forceinline__ V8 ld_stream_ordered(const void* p) {
+  V8 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "l"(p));
   return v;
 }
@@ -63,6 +80,12 @@ template <> struct VecOf<32> { typedef V16 type; };
 __device__ __forceinline__ V16 ld_stream32(const void* p) {
   V16 v;
   asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7]) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ V16 ld_stream32_ordered(const void* p) {
+  V16 v;
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7]) : "l"(p));
   return v;
 }

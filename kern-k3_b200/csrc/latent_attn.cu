@@ -282,13 +282,13 @@ struct Loader {
       const unsigned char* src = w.page + (token & 63) * (MX8 ? kLatent : 2 * kRow) + block * (MX8 ? 32 : 64);
       if (MX8 && P0 == 0) {
         const unsigned char* sc = w.page + kPageScales + (token & 63) * (kLatent / 32);
-        scales[0] = ld_stream(sc);
-        scales[1] = ld_stream(sc + 8 * (kLatent / 32));
+        scales[0] = ld_stream_ordered(sc);
+        scales[1] = ld_stream_ordered(sc + 8 * (kLatent / 32));
       }
 #pragma unroll
       for (int p = P0; p < P1; ++p)
 #pragma unroll
-        for (int g = 0; g < 2; ++g) code[p][g] = ld_stream32(src + (MX8 ? p * 128 + g * 8 * kLatent : (p >> 1) * 256 + (p & 1) * 32 + g * 16 * kRow));
+        for (int g = 0; g < 2; ++g) code[p][g] = ld_stream32_ordered(src + (MX8 ? p * 128 + g * 8 * kLatent : (p >> 1) * 256 + (p & 1) * 32 + g * 16 * kRow));
     } else {
       if (P0 == 0) scales[0] = scales[1] = V8{{0u, 0u, 0u, 0u}};
 #pragma unroll
@@ -507,13 +507,14 @@ __device__ __forceinline__ void fetch_q(const AttnArgs& a, Control& k, const Seg
   const int r = tid >> 2;
   const __nv_bfloat16* src = query(a, s, r);
   const uint4* from = reinterpret_cast<const uint4*>(src) + (tid & 3);
+  auto read = [](const uint4* p) { const V8 v = ld_plain(p); return make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]); };
   const __nv_bfloat16* rope_src = query(a, s, tid & 63);
   uint4 x[16];
   unsigned top = 0, rope[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     if (MX8) {
-      x[i] = src ? __ldg(from + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
+      x[i] = src ? read(from + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
     } else {
       const int unit = 4 * i + (tid & 3);
       copy16(q + (unit >> 3) * kQChunk + unit_at(r, unit & 7), reinterpret_cast<const unsigned char*>(src ? from + 4 * i : reinterpret_cast<const uint4*>(a.q)), src != nullptr);
@@ -522,7 +523,7 @@ __device__ __forceinline__ void fetch_q(const AttnArgs& a, Control& k, const Seg
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 y = rope_src ? __ldg(reinterpret_cast<const uint4*>(rope_src + kLatent + (tid >> 7) * 32) + i) : make_uint4(0u, 0u, 0u, 0u);
+    const uint4 y = rope_src ? read(reinterpret_cast<const uint4*>(rope_src + kLatent + (tid >> 7) * 32) + i) : make_uint4(0u, 0u, 0u, 0u);
     rope[4 * i] = y.x; rope[4 * i + 1] = y.y; rope[4 * i + 2] = y.z; rope[4 * i + 3] = y.w;
   }
   float up = 1.f;
@@ -782,7 +783,7 @@ __device__ void plan(const AttnArgs& a, Control& k, int ptok, int page_bytes, in
 #pragma unroll 1
     for (int t = s.t0; t < s.t1; ++t, ++i) {
       const int off = (t - s.t0) * 2 % 32;
-      if (off == 0) ids = 2 * t + lane < pages ? __ldg(table + 2 * t + lane) : -1;
+      if (off == 0) ids = 2 * t + lane < pages ? ld_ordered(table + 2 * t + lane) : -1;
       Tile w;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {

@@ -20,19 +20,19 @@ namespace {
 
 constexpr int kWarps = 8;
 
-__global__ void __launch_bounds__(32 * kWarps) latent_mx8_store_kernel(const __nv_bfloat16* __restrict__ rows, long long row_stride,
-                                                                       const long long* __restrict__ slot_mapping,
-                                                                       unsigned char* __restrict__ cache, long long page_stride,
+__global__ void __launch_bounds__(32 * kWarps) latent_mx8_store_kernel(const __nv_bfloat16* rows, long long row_stride,
+                                                                       const long long* slot_mapping,
+                                                                       unsigned char* cache, long long page_stride,
                                                                        long long slots, int T) {
   const int lane = threadIdx.x & 31;
   const long long t = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
   follow_launch();
   if (t >= T) return;
-  const long long slot = __ldg(slot_mapping + t);
+  const long long slot = ld_ordered(slot_mapping + t);
   const __nv_bfloat16* row = rows + t * row_stride;
-  const V8 a = ld_stream(row + 16 * lane), b = ld_stream(row + 16 * lane + 8);
+  const V8 a = ld_stream_ordered(row + 16 * lane), b = ld_stream_ordered(row + 16 * lane + 8);
   V8 r;
-  if (lane < 8) r = ld_stream(row + kLatent + 8 * lane);
+  if (lane < 8) r = ld_stream_ordered(row + kLatent + 8 * lane);
   unsigned m = max_bf16_bits(absmax8(a), absmax8(b));
   m = max_bf16_bits(m, __shfl_xor_sync(0xffffffffu, m, 1));
   const int e = ue8m0_exp_from_bf16(m);
@@ -48,22 +48,22 @@ __global__ void __launch_bounds__(32 * kWarps) latent_mx8_store_kernel(const __n
   if ((lane & 1) == 0) page[kPageScales + at * (kLatent / 32) + (lane >> 1)] = (unsigned char)(e + 127);
 }
 
-__global__ void __launch_bounds__(32 * kWarps) latent_mx8_gather_kernel(const unsigned char* __restrict__ cache, const int* __restrict__ block_table,
-                                                                        long long page_stride, long long pages, const int* __restrict__ lens,
-                                                                        __nv_bfloat16* __restrict__ out, int n) {
+__global__ void __launch_bounds__(32 * kWarps) latent_mx8_gather_kernel(const unsigned char* cache, const int* block_table,
+                                                                        long long page_stride, long long pages, const int* lens,
+                                                                        __nv_bfloat16* out, int n) {
   const int lane = threadIdx.x & 31;
   follow_launch();
   const int len = ld_ordered(lens);
   const long long t = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (t >= n) return;
   V8 a = {{0u, 0u, 0u, 0u}}, b = a, r = a;
-  const int id = t < len ? __ldg(block_table + (t >> 6)) : -1;
+  const int id = t < len ? ld_ordered(block_table + (t >> 6)) : -1;
   if (id >= 0 && id < pages) {
     const unsigned char* page = cache + id * page_stride;
     const int at = (int)(t & 63);
-    const V8 q = ld_stream(page + at * kLatent + 16 * lane);
-    if (lane < 8) r = ld_stream(page + kPageRope + at * (2 * kRopeCols) + 16 * lane);
-    const unsigned s = ue8m0_pair(__ldg(page + kPageScales + at * (kLatent / 32) + (lane >> 1)));
+    const V8 q = ld_stream_ordered(page + at * kLatent + 16 * lane);
+    if (lane < 8) r = ld_stream_ordered(page + kPageRope + at * (2 * kRopeCols) + 16 * lane);
+    const unsigned s = ue8m0_pair(ld_ordered(page + kPageScales + at * (kLatent / 32) + (lane >> 1)));
     mx8_to_bf16x4(q.w[0], s, a.w[0], a.w[1]);
     mx8_to_bf16x4(q.w[1], s, a.w[2], a.w[3]);
     mx8_to_bf16x4(q.w[2], s, b.w[0], b.w[1]);

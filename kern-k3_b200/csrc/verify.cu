@@ -37,17 +37,17 @@ __device__ __forceinline__ double weight(float p, float q) {
   const double d = (double)p - (double)q;
   return d > 0.0 && d < (double)INFINITY ? d : 0.0;          // NaN and infinite entries weigh nothing
 }
-__device__ __forceinline__ float q_at(const Rows& r, int v) { return r.q ? __ldg(r.q + v) : (v == r.hot ? 1.f : 0.f); }
+__device__ __forceinline__ float q_at(const Rows& r, int v) { return r.q ? k3g::ld_ordered(r.q + v) : (v == r.hot ? 1.f : 0.f); }
 
 // Weights of elements v .. v + 3 (those below `end`).
 template <bool VEC>
 __device__ __forceinline__ void weights4(const Rows& r, int v, int end, double (&w)[4]) {
   float p[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
   if (VEC && v + 4 <= end) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(r.p + v));
+    const float4 a = k3g::ld_ordered(reinterpret_cast<const float4*>(r.p + v));
     p[0] = a.x; p[1] = a.y; p[2] = a.z; p[3] = a.w;
     if (r.q) {
-      const float4 b = __ldg(reinterpret_cast<const float4*>(r.q + v));
+      const float4 b = k3g::ld_ordered(reinterpret_cast<const float4*>(r.q + v));
       q[0] = b.x; q[1] = b.y; q[2] = b.z; q[3] = b.w;
     } else {
 #pragma unroll
@@ -56,7 +56,7 @@ __device__ __forceinline__ void weights4(const Rows& r, int v, int end, double (
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (v + j < end) { p[j] = __ldg(r.p + v + j); q[j] = q_at(r, v + j); }
+      if (v + j < end) { p[j] = k3g::ld_ordered(r.p + v + j); q[j] = q_at(r, v + j); }
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) w[j] = weight(p[j], q[j]);
@@ -108,8 +108,8 @@ __device__ __noinline__ double segment_sum(const Rows r, int lo, int hi, int lan
       float4 p[kBatch], q[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        p[j] = __ldg(reinterpret_cast<const float4*>(r.p + v + 128 * j));
-        q[j] = __ldg(reinterpret_cast<const float4*>(r.q + v + 128 * j));
+        p[j] = k3g::ld_ordered(reinterpret_cast<const float4*>(r.p + v + 128 * j));
+        q[j] = k3g::ld_ordered(reinterpret_cast<const float4*>(r.q + v + 128 * j));
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) s += (weight(p[j].x, q[j].x) + weight(p[j].y, q[j].y)) + (weight(p[j].z, q[j].z) + weight(p[j].w, q[j].w));
@@ -153,10 +153,10 @@ __device__ __forceinline__ int segment_find(const Rows& r, int lo, int hi, doubl
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const float* __restrict__ target, long long target_stride,
-                                                                const float* __restrict__ draft, long long draft_stride,
-                                                                const long long* __restrict__ ids, const float* __restrict__ u,
-                                                                int* __restrict__ accepted, long long* __restrict__ tokens, int S, int V,
+__global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const float* target, long long target_stride,
+                                                                const float* draft, long long draft_stride,
+                                                                const long long* ids, const float* u,
+                                                                int* accepted, long long* tokens, int S, int V,
                                                                 int slice) {
   __shared__ double s_sum[kSegs];
   __shared__ double s_all[kMaxCluster * kSegs];
@@ -168,12 +168,12 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const float* 
   // every warp decides for itself which drafts stay
   bool valid = false, keep = false;
   if (lane < S) {
-    const long long x = ids[(long long)b * S + lane];
+    const long long x = k3g::ld_ordered(ids + (long long)b * S + lane);
     valid = x >= 0 && x < V;
     if (valid) {
-      const double px = target[((long long)b * (S + 1) + lane) * target_stride + x];
-      const double qx = draft ? (double)draft[((long long)b * S + lane) * draft_stride + x] : 1.0;
-      keep = (double)u[(long long)b * (S + 1) + lane] * qx < px;
+      const double px = k3g::ld_ordered(target + ((long long)b * (S + 1) + lane) * target_stride + x);
+      const double qx = draft ? (double)k3g::ld_ordered(draft + ((long long)b * S + lane) * draft_stride + x) : 1.0;
+      keep = (double)k3g::ld_ordered(u + (long long)b * (S + 1) + lane) * qx < px;
     }
   }
   const unsigned kept_mask = __ballot_sync(0xffffffffu, valid && keep), valid_mask = __ballot_sync(0xffffffffu, valid);
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const float* 
   Rows r;
   r.p = target + ((long long)b * (S + 1) + kept) * target_stride;
   r.q = turned_down && draft ? draft + ((long long)b * S + kept) * draft_stride : nullptr;
-  r.hot = turned_down && !draft ? (int)ids[(long long)b * S + kept] : -1;
+  r.hot = turned_down && !draft ? (int)k3g::ld_ordered(ids + (long long)b * S + kept) : -1;
 
   // the slice of this block, one contiguous segment (a multiple of 4 elements) for each warp
   const int seg = (slice / kSegs);
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const float* 
     r.q = nullptr; r.hot = -1;                               // p <= q everywhere: draw from p
   }
   // the segment that holds the point: the first whose running sum passes it, else the last that weighs anything
-  const double point = (double)u[(long long)b * (S + 1) + S] * total;
+  const double point = (double)k3g::ld_ordered(u + (long long)b * (S + 1) + S) * total;
   double base;
   const int pick_seg = part_of(part, upto, point, lane, base);
   if (rank != (pick_seg < 0 ? 0 : pick_seg / kSegs)) return;
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draft_kernel(const float* 
   if (mine) {
     if (lane == 0) accepted[b] = kept;
     for (int i = lane; i <= S; i += 32)
-      tokens[(long long)b * (S + 1) + i] = i < kept ? ids[(long long)b * S + i] : i == kept ? (long long)pick : -1ll;
+      tokens[(long long)b * (S + 1) + i] = i < kept ? k3g::ld_ordered(ids + (long long)b * S + i) : i == kept ? (long long)pick : -1ll;
   }
 }
 

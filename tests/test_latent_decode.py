@@ -581,3 +581,55 @@ def test_decode_steps_with_drafts_over_one_prompt(k3g, dev):
         assert torch.equal(base, before + accepted + 1)
         total += int(accepted.sum())
     assert int(base.max()) > 64
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_launched_behind_one_another_each_reads_what_the_one_before_wrote(k3g, dev, captured):
+    """A chain without a wait of the host's: the token that verification draws is the slot of the row stored next, the cache is read back, attended to,
+    and 150 times so, every time another row over the same pages.  Each output is what the same calls give with a wait after each."""
+    import torch
+    g = rng(34)
+    pages, n, heads = 3, 150, 8
+    V = pages * 64
+    rows = to_dev_bf16(normal_bf16(g, (n, ROW)), dev)
+    u = torch.rand((n, 1), device=dev, generator=torch.Generator(device=dev).manual_seed(34))
+    target = torch.full((1, 1, V), 1.0 / V, device=dev)
+    q = to_dev_bf16(normal_bf16(g, (1, 1, heads, ROW)), dev)
+    table, lens = torch.tensor([2, 0, 1], dtype=torch.int32, device=dev), torch.tensor([V], dtype=torch.int32, device=dev)
+    start = torch.zeros(pages * MX8_PAGE, dtype=torch.uint8, device=dev)
+    k3g.call("k3g_latent_mx8_store", to_dev_bf16(normal_bf16(g, (V, ROW)), dev), ROW, torch.arange(V, device=dev), start, 0, MX8_PAGE, pages, V, k3g.current_stream())
+    cache = torch.empty_like(start)
+    accepted, token = torch.empty(1, dtype=torch.int32, device=dev), torch.empty((1, 1), dtype=torch.int64, device=dev)
+    ws = torch.empty(k3g.latent_attn_workspace(1, 1, heads), dtype=torch.uint8, device=dev)
+
+    def chain(tokens, back, out, stop):
+        cache.copy_(start)
+        for i in range(n):
+            s = k3g.current_stream()
+            k3g.call("k3g_verify_draft", target, V, None, V, token, u[i], accepted, token, 1, 0, V, s)
+            stop()
+            k3g.call("k3g_latent_mx8_store", rows[i], ROW, token, cache, 0, MX8_PAGE, pages, 1, s)
+            stop()
+            k3g.call("k3g_latent_mx8_gather", cache, table, 0, MX8_PAGE, pages, lens, back[i], V, s)
+            stop()
+            k3g.call("k3g_latent_attn", q, heads * ROW, cache, 1, 0, MX8_PAGE, pages, None, None, 0, table, lens, pages, out[i], ws, ws.numel(), 1, 1, heads, 0.07, s)
+            stop()
+            tokens[i].copy_(token.view(-1))
+
+    def outputs():
+        return (torch.zeros((n, 1), dtype=torch.int64, device=dev), torch.zeros((n, V, ROW), dtype=torch.bfloat16, device=dev),
+                torch.zeros((n, heads, LATENT), dtype=torch.bfloat16, device=dev))
+    want, got = outputs(), outputs()
+    chain(*want, torch.cuda.synchronize)
+    torch.cuda.synchronize()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            chain(*got, lambda: None)
+        graph.replay()
+    else:
+        chain(*got, lambda: None)
+    torch.cuda.synchronize()
+    assert len(torch.unique(want[0])) > 50
+    for a, b in zip(want, got):
+        assert torch.equal(a.view(torch.int64 if a.dtype == torch.int64 else torch.int16), b.view(torch.int64 if b.dtype == torch.int64 else torch.int16))

@@ -124,3 +124,15 @@ def test_warps_shares_of_registers_are_what_the_attention_is_launched_with(tmp_p
     threads = sizes["kSoftmax"] + sizes["kLoaders"] + 128
     for n in used:
         assert sizes["kSoftmax"] * softmax + sizes["kLoaders"] * loaders + 128 * rest <= threads * ((n + 7) // 8 * 8)
+
+
+@pytest.mark.parametrize("name", ["latent_attn.cu", "latent_cache.cu", "latent_page.cuh", "verify.cu"])
+def test_kernels_launched_behind_others_load_coherently(name):
+    """They begin while the launch before them still writes: nothing that they read is read-only for as long as they run, so no load of theirs may take
+    the path that asks for it (nor be given it by the compiler, for const __restrict__)."""
+    import os
+    import re
+    here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    source = open(os.path.join(here, "kern-k3_b200", "csrc", name)).read()
+    source = re.sub(r"//[^\n]*", "", source)
+    assert not re.findall(r"__ldg\b|ld\.global\.nc|ld_stream(?:32|_vec<\d+>)?\(|ld_keep\w*|__restrict__", source)

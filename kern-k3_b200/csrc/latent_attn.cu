@@ -338,6 +338,25 @@ struct Loader {
     if ((token & 63) + 8 * g >= here.tokens) o.u[0] = o.u[1] = o.u[2] = o.u[3] = make_uint4(0u, 0u, 0u, 0u);
     return o;
   }
+  // The largest scale byte again, of blocks that are not all zeros: those have byte 127 whatever lies beside them, and where the others' are below it
+  // it would take the range from them.  The thread's own blocks of zeros have a factor of 0 from here on.  Run only where 127 is the largest byte: ordinary
+  // latents, whose blocks hold magnitudes up to 224, get there through a block of zeros alone.
+  __device__ __forceinline__ unsigned most_of_blocks() {
+    unsigned most = 0;
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const unsigned byte = (scales[g].w[p] >> (block * 8)) & 0xffu;
+        unsigned any = 0;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) any |= code[p][g].w[x];
+        if (byte == 255) continue;                           // NaN, whatever the codes are
+        if ((any & 0x7f7f7f7fu) == 0) scales[g].w[p] &= ~(0xffu << (block * 8));
+        else if ((token & 63) + 8 * g < here.tokens) most = max(most, byte + 1);
+      }
+    return __reduce_max_sync(0xffffffffu, most);
+  }
   unsigned bad[2];                                           // the thread's tokens have values that are not finite
   __device__ __forceinline__ void put(int p, int g, const Units& o) {
 #pragma unroll
@@ -364,7 +383,9 @@ struct Loader {
         asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(((w & 0x00ff00ffu) + 0x00010001u) & 0x00ff00ffu), "r"((((w >> 8) & 0x00ff00ffu) + 0x00010001u) & 0x00ff00ffu));
         if ((token & 63) + 8 * g < here.tokens) most = max(most, max(m & 0xffffu, m >> 16));
       }
-      most = min(max(__reduce_max_sync(0xffffffffu, most), (unsigned)(128 + kLeastE)), (unsigned)(128 + kMostE)) - 1;
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (most == 128) most = most_of_blocks();
+      most = min(max(most, (unsigned)(128 + kLeastE)), (unsigned)(128 + kMostE)) - 1;
     }
     Units u = convert(0, 0, most), v = convert(0, 1, most);
     empty(i, 0);

@@ -419,6 +419,61 @@ def test_attn_workspace_of_a_larger_batch_serves_a_smaller_one(k3g, dev):
     c.compare(bf16_bits(c.out))
 
 
+# ---- exponents of MXFP8 pages ------------------------------------------------------------------------------------------------
+def _fill(c, rows):
+    """The whole cache of an MXFP8 case from rows [pages * 64, 576] of floats."""
+    c.rows = rows
+    q, rope, sf = quant_rows(k3o.f32_to_bf16(rows.astype(np.float32).reshape(-1)).reshape(rows.shape))
+    at = c.cache.reshape(c.pages, c.stride)[:, c.off:c.off + MX8_PAGE]
+    at[:, :ROPE_AT] = q.reshape(c.pages, -1)
+    at[:, ROPE_AT:SCALES_AT] = np.ascontiguousarray(rope).view(np.uint8).reshape(c.pages, -1)
+    at[:, SCALES_AT:] = sf.reshape(c.pages, -1)
+    return c
+
+
+def _token(table, t):
+    return int(table[t // 64]) * 64 + t % 64
+
+
+@pytest.mark.parametrize("where", ["row beside", "block beside", "sixteen rows", "rows of another tile", "every other row"])
+@pytest.mark.parametrize("size", [-10, -20, -30])
+def test_attn_mx8_zeros_beside_small_latents(k3g, dev, size, where):
+    """A block of zeros has scale byte 127 whatever lies beside it: it takes nothing from the range of the tokens that are not zero."""
+    c = Case(dev, 2, 2, 12, 300, [70, 200], seed=40 - size)
+    rows = normal_bf16(c.g, (c.pages * 64, ROW))
+    rows = k3o.bf16_to_f32(rows.reshape(-1)).reshape(rows.shape).copy()
+    rows[:, :LATENT] *= 2.0 ** size
+    p = c.prefix_table
+    if where == "row beside":
+        rows[[_token(p, 5), _token(c.tables[0], 66), _token(c.tables[1], 199)], :LATENT] = 0
+    elif where == "block beside":
+        rows[[_token(p, t) for t in range(3, 300, 16)], 64:96] = 0
+        rows[_token(c.tables[1], 130), 480:512] = -0.0
+    elif where == "sixteen rows":
+        rows[[_token(p, t) for t in range(16, 32)], :LATENT] = 0
+    elif where == "rows of another tile":
+        rows[[_token(p, t) for t in range(256, 300)], :LATENT] = 0
+        rows[[_token(c.tables[1], t) for t in range(128)], :LATENT] = -0.0
+    else:
+        rows[::2, :LATENT] = 0
+    _fill(c, rows).check(k3g)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_attn_mx8_a_nan_scale_over_codes_of_zero(k3g, dev, zeros):
+    """Scale byte 255 is NaN whatever it scales, with a block of zeros among the sixteen tokens and without."""
+    c = Case(dev, 2, 1, 12, 0, [70, 30], seed=45)
+    t = _token(c.tables[0], 20)
+    if zeros:
+        c.set_token(c.tables[0], 19, np.zeros(ROW, dtype=np.uint16))
+    page = c.cache.reshape(c.pages, c.stride)[t // 64, c.off:]
+    page[t % 64 * LATENT + 96:t % 64 * LATENT + 128] = 0
+    page[SCALES_AT + t % 64 * 16 + 3] = 255
+    c.check(k3g)
+    want, _, _ = c.oracle()
+    assert np.isnan(want[0]).all() and np.isfinite(want[1]).all()
+
+
 # ---- verification ------------------------------------------------------------------------------------------------------------
 def _probs(g, shape, std=2.5):
     x = g.standard_normal(shape) * std

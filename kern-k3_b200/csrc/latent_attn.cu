@@ -37,12 +37,13 @@
 //
 // Types.  bf16 pages are multiplied as bf16.  MXFP8 codes become f16, not bf16: one conversion and one product for two codes, a third of what bf16
 // takes (which has no conversion from E4M3), and the loaders' instructions are what a tile waits for.  f16 has the bits (a code has four), but not the
-// range, so exponents are taken out: of the scales of 16 tokens the largest, E (K' = code * 2^(e - E), exact down to 2^-24 of 2^E), of
-// a query row its own (the largest element is brought to 2^14..2^15; what that costs is below 2^-39 of it).  They come back in f32: S = 2^(E + row) S' + S_rope
+// range, so exponents are taken out: of the scales of 16 tokens (but those of blocks of zeros) the largest less kRoom, E (K' = code * 2^(e - E): blocks whose
+// scale is 2^-32 of the largest become 0, others keep what is above 2^-24 of 2^E, 2^-39 of the largest element), of a query row its own (the largest element
+// is brought to 2^14..2^15; what that costs is below 2^-39 of it).  They come back in f32: S = 2^(E + row) S' + S_rope
 // (the rope columns are multiplied as bf16 into a second accumulator), and P' = 2^(S + E - m), with m the running maximum of S + E, so
 // that P' V' has the weight of P V.  P is rounded because both operands of the matrix instructions are 16 bits; the sums of P stay unrounded in f32.
 // The m that P' is relative to follows the true maximum only when it falls behind by more than 2^4 (O is then rescaled): the ratio is
-// exact either way.  P' is kept in 2^-24 .. 2^14, with 2^10 at the maximum: tokens are lost below 2^-34 of the largest.
+// exact either way.  P' is kept in 2^-24 .. 2^14, with 2^10 at the maximum: tokens whose weight times 2^E is below 2^-34 of the largest such product are lost.
 #include <cuda_runtime.h>
 
 #include "latent_page.cuh"
@@ -60,7 +61,8 @@ constexpr int kSmemQ = 8 * kQChunk, kSmemP = 2 * kQChunk, kSmemK = 9 * kChunk, k
 // tensor memory columns: O 0..255 (four accumulators of 128 output columns, 64 on either half of the lanes), S 256..319 (a page on either
 // half), the rope columns' part of S 320..383 (MXFP8), the queries' rope columns 384..415 (the same on both halves)
 constexpr int kTmemS = 256, kTmemR = 320, kTmemQ = 384;
-constexpr int kLeastE = -80, kMostE = 120;                   // exponents of 16 tokens: sums of 2^-E stay in range
+constexpr int kRoom = 7;                                     // E is the largest scale's exponent less this: codes reach 448 = 2^8.8, f16 2^16
+constexpr int kLeastE = -80;                                 // sums of 2^-E stay in range (E is 120 at most)
 constexpr float kLag = 4.f, kTop = 10.f;                     // the long document above 340 us when it was chosen, with a lag of 0 (O rescaled for every new maximum) 359
 constexpr int kPartFloats = kRows * kLatent;                 // a part's outputs; its 64 (maximum, sum) pairs lie in a table of their own
 constexpr int kWaitLimit = 1 << 20, kRing = 4, kReaders = kSoftmax / 32 + 1, kTiles = 2;
@@ -219,11 +221,13 @@ __device__ __forceinline__ uint4 load16(unsigned at) {
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_left() { asm volatile("cp.async.wait_group %0;" :: "n"(LEFT) : "memory"); }
 
-// 2^(byte - most) as a pair of f16 (byte 255: NaN), and four E4M3 codes times it: exact but for what falls below f16's 2^-24.
-__device__ __forceinline__ unsigned f16_scale(unsigned most, unsigned byte) {
-  const float f = __uint_as_float((unsigned)max((int)(byte + 127 - most), 0) << 23);
-  const __half2 h = __floats2half2_rn(f, f);
-  return byte == 255 ? 0x7e007e00u : *reinterpret_cast<const unsigned*>(&h);
+// 2^(byte - base) as a pair of f16 (byte 255: NaN), and four E4M3 codes times it.  Scales are 2^kRoom times the base at most, and 448 * 2^kRoom is below f16's
+// largest; from 2^-24 up the factor is one of f16's, and the product is exact but for what falls below 2^-24.  A block of zeros may have any byte: a
+// factor that f16 does not hold is cut to its largest.
+__device__ __forceinline__ unsigned f16_scale(unsigned base, unsigned byte) {
+  unsigned h;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %1;" : "=r"(h) : "f"(__uint_as_float((unsigned)max((int)(byte + 127 - base), 0) << 23)));
+  return byte == 255 ? 0x7e007e00u : h;
 }
 __device__ __forceinline__ void mx8_to_f16x4(unsigned codes, unsigned scale, unsigned& lo, unsigned& hi) {
   asm("{.reg .b16 a, b; .reg .b32 x, y; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 x, a; cvt.rn.f16x2.e4m3x2 y, b; mul.rn.f16x2 %0, x, %3; mul.rn.f16x2 %1, y, %3;}"
@@ -339,9 +343,9 @@ struct Loader {
     return o;
   }
   // The largest scale byte again, of blocks that are not all zeros: those have byte 127 whatever lies beside them, and where the others' are below it
-  // it would take the range from them.  The thread's own blocks of zeros have a factor of 0 from here on.  Run only where 127 is the largest byte: ordinary
-  // latents, whose blocks hold magnitudes up to 224, get there through a block of zeros alone.
-  __device__ __forceinline__ unsigned most_of_blocks() {
+  // it would take the range from them.  Run only where 127 is the largest byte: latents whose blocks hold magnitudes up to 224 get there through a block
+  // of zeros alone.
+  __device__ __forceinline__ unsigned most_of_blocks() const {
     unsigned most = 0;
 #pragma unroll
     for (int p = 0; p < 4; ++p)
@@ -351,9 +355,7 @@ struct Loader {
         unsigned any = 0;
 #pragma unroll
         for (int x = 0; x < 8; ++x) any |= code[p][g].w[x];
-        if (byte == 255) continue;                           // NaN, whatever the codes are
-        if ((any & 0x7f7f7f7fu) == 0) scales[g].w[p] &= ~(0xffu << (block * 8));
-        else if ((token & 63) + 8 * g < here.tokens) most = max(most, byte + 1);
+        if (byte != 255 && (any & 0x7f7f7f7fu) != 0 && (token & 63) + 8 * g < here.tokens) most = max(most, byte + 1);
       }
     return __reduce_max_sync(0xffffffffu, most);
   }
@@ -385,7 +387,7 @@ struct Loader {
       }
       most = __reduce_max_sync(0xffffffffu, most);
       if (most == 128) most = most_of_blocks();
-      most = min(max(most, (unsigned)(128 + kLeastE)), (unsigned)(128 + kMostE)) - 1;
+      most = (unsigned)max((int)most - 1 - kRoom, 127 + kLeastE);
     }
     Units u = convert(0, 0, most), v = convert(0, 1, most);
     empty(i, 0);

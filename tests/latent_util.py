@@ -102,6 +102,41 @@ def attn_tolerance(out, spread, ds):
     return 2.0 ** -8 * np.abs(out) + (2.0 ** -8 + 2.0 ** -10 + 3 * d) * spread + 1e-30
 
 
+def mx8_range_tolerance(q, rows_of, prefix_table, prefix_len, tables, lens, scale):
+    """What k3g_latent_attn may lose beside attn_tolerance because MXFP8 pages and queries are multiplied as f16: (of the outputs, of the
+    scores), per row.  M is the largest latent magnitude of the 16 tokens around one.
+      an element below 2^-31 M may count as 0, one that does not is off by less: 2^-31 sum_j p_j M_j in the outputs, scale * 2^-31 M
+      sum |q| in a score;
+      a token's weight is off by 2^-25 where the largest weight * 2^E is 2^10 or more, and M is in (224, 448] 2^E: 2^-34 max_j p_j M_j for
+      each token (twice that where E is what a neighbour's block, rounded up to it, gives);
+      a query's element below 2^-39 of its row's largest may count as 0: scale * 2^-39 max |q| sum |k| in a score."""
+    B, S, H, _ = q.shape
+    lost, dlost = np.zeros((B, S, H)), np.zeros((B, S, H))
+
+    def read(table, n):
+        k, held = rows_of(table, n)
+        big = np.zeros(n)
+        for t in range(0, n, 16):
+            big[t:t + 16] = np.abs(k[t:t + 16, :LATENT]).max()
+        return k[held], big[held]
+    empty = np.zeros((0, ROW)), np.zeros(0)
+    pk, pm = read(prefix_table, prefix_len) if prefix_len > 0 else empty
+    for b in range(B):
+        sk, sm = read(tables[b], int(lens[b])) if lens[b] > 0 else empty
+        for s in range(S):
+            n = max(0, int(lens[b]) - (S - 1 - s))
+            k, m = np.concatenate([pk, sk[:n]]), np.concatenate([pm, sm[:n]])
+            if not len(k):
+                continue
+            x = scale * (q[b, s] @ k.T)
+            p = np.exp(x - x.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            lost[b, s] = 2.0 ** -31 * (p @ m) + 2.0 ** -33 * len(k) * (p * m).max(1)
+            lat = np.abs(q[b, s, :, :LATENT])
+            dlost[b, s] = abs(scale) * (2.0 ** -31 * m.max() * lat.sum(1) + 2.0 ** -39 * lat.max(1) * np.abs(k[:, :LATENT]).sum(1).max())
+    return lost, dlost
+
+
 def verify_oracle(target, draft, ids, u):
     """(accepted, tokens) of k3g_verify_draft; target [B, S + 1, V], draft [B, S, V] or None."""
     B, S = ids.shape

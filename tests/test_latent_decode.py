@@ -3,8 +3,8 @@ import numpy as np
 import pytest
 
 import k3o
-from latent_util import (LATENT, MX8_PAGE, PAGE, ROPE_AT, ROW, SCALES_AT, attn_oracle, attn_tolerance, bf16_rows, mx8_rows, put_rows, quant_rows,
-                         verify_oracle)
+from latent_util import (LATENT, MX8_PAGE, PAGE, ROPE_AT, ROW, SCALES_AT, attn_oracle, attn_tolerance, bf16_rows, mx8_range_tolerance, mx8_rows, put_rows,
+                         quant_rows, verify_oracle)
 from util import bf16_bits, normal_bf16, rng, to_dev, to_dev_bf16
 
 pytestmark = pytest.mark.gpu
@@ -472,6 +472,52 @@ def test_attn_mx8_a_nan_scale_over_codes_of_zero(k3g, dev, zeros):
     c.check(k3g)
     want, _, _ = c.oracle()
     assert np.isnan(want[0]).all() and np.isfinite(want[1]).all()
+
+
+def _scale_q(c, heads):
+    """Latent columns of the queries times a factor for each head (powers of two, or 0)."""
+    f = k3o.bf16_to_f32(np.ascontiguousarray(c.q)).reshape(c.B, c.S, c.heads, ROW)
+    f[..., :LATENT] *= np.asarray(heads, dtype=np.float32).reshape(-1, 1)
+    c.q = k3o.f32_to_bf16(f.reshape(-1)).reshape(c.q.shape)
+
+
+def _check_range(c, k3g):
+    """As Case.check, with what f16 operands may lose beside it."""
+    import torch
+    c.upload(k3g).call(k3g)
+    torch.cuda.synchronize()
+    got = k3o.bf16_to_f32(bf16_bits(c.out)).astype(np.float64)
+    want, spread, ds = c.oracle()
+    q = k3o.bf16_to_f32(np.ascontiguousarray(c.q)).astype(np.float64).reshape(c.B, c.S, c.heads, ROW)
+    lost, dlost = mx8_range_tolerance(q, lambda t, n: mx8_rows(c.cache, c.off, c.stride, t, n), c.prefix_table, c.prefix, c.tables, c.lens, c.scale)
+    off = np.abs(got - want) - attn_tolerance(want, spread, ds) - 3 * dlost[..., None] * spread - lost[..., None]
+    assert np.all(off <= 0), "worst excess %g" % off.max()
+
+
+@pytest.mark.parametrize("scale", [0.07, -0.07])
+@pytest.mark.parametrize("kind", ["blocks", "blocks upwards", "tokens", "tiles", "pages of 2^-30", "tiles of 2^20"])
+def test_attn_mx8_magnitudes_that_differ(k3g, dev, kind, scale):
+    """Scales that spread over 2^30 and more within a token, within 16 tokens and from tile to tile."""
+    c = Case(dev, 2, 2, 12, 700, [70, 200], seed=50, scale=scale)
+    rows = normal_bf16(c.g, (c.pages * 64, ROW))
+    rows = k3o.bf16_to_f32(rows.reshape(-1)).reshape(rows.shape).copy()
+    token, block = np.arange(c.pages * 64)[:, None], np.arange(LATENT)[None] // 32
+    if kind == "blocks":
+        up = -np.round(2.2 * block) + 0 * token                  # 0 .. -33
+    elif kind == "blocks upwards":
+        up = np.round(1.4 * block) - 20 + token % 3 - 1          # the last block largest
+    elif kind == "tokens":
+        up = (token * 7 % 16) * -2 + 0 * block                   # 0 .. -30
+    elif kind == "tiles":
+        up = c.g.integers(-20, 21, c.pages)[token // 64] + 0 * block
+    elif kind == "pages of 2^-30":
+        up = np.where(token // 64 % 2 == 0, -30, 0) + 0 * block
+    else:
+        up = np.where(token // 128 % 3 == 1, 20, 0) + 0 * block
+    rows[:, :LATENT] *= 2.0 ** up
+    rows[::37, :LATENT] = 0
+    _scale_q(c, [2.0 ** -max(0, int(up.max()))] * c.heads)
+    _check_range(_fill(c, rows), k3g)
 
 
 # ---- verification ------------------------------------------------------------------------------------------------------------

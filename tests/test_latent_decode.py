@@ -520,6 +520,55 @@ def test_attn_mx8_magnitudes_that_differ(k3g, dev, kind, scale):
     _check_range(_fill(c, rows), k3g)
 
 
+@pytest.mark.parametrize("size", [-90, -75, 60, 115])
+def test_attn_mx8_latents_at_the_ends_of_the_exponents(k3g, dev, size):
+    """Latents of 2^-90 (where E has reached its least) to 2^115, queries that make scores of ordinary size of them, zeros among them."""
+    c = Case(dev, 2, 2, 12, 150, [70, 130], seed=55, scale=0.07)
+    rows = normal_bf16(c.g, (c.pages * 64, ROW))
+    rows = k3o.bf16_to_f32(rows.reshape(-1)).reshape(rows.shape).copy()
+    rows[:, :LATENT] *= np.float32(2.0 ** size)
+    rows[::23, :LATENT] = 0
+    _scale_q(c, [2.0 ** -size] * c.heads)
+    _check_range(_fill(c, rows), k3g)
+
+
+@pytest.mark.parametrize("scale", [0.07, -0.07])
+@pytest.mark.parametrize("size", [-40, 0, 12])
+def test_attn_mx8_query_rows_of_any_size(k3g, dev, size, scale):
+    """Queries from 2^-40 to 2^40 beside one another, rows of zeros among them, so that scores count at one end."""
+    c = Case(dev, 3, 2, 11, 260, [5, 70, 128], seed=60 + size, scale=scale)
+    rows = normal_bf16(c.g, (c.pages * 64, ROW))
+    rows = k3o.bf16_to_f32(rows.reshape(-1)).reshape(rows.shape).copy()
+    rows[:, :LATENT] *= 2.0 ** size
+    heads = [2.0 ** (10 * h - 40) if 10 * h - 40 <= -size else 0.0 for h in range(9)] + [0.0, 2.0 ** -size]
+    _scale_q(c, heads)
+    c.q.reshape(c.B, c.S, c.heads, ROW)[:, 0, 9] = 0             # zeros in the rope columns, too
+    c.q.reshape(c.B, c.S, c.heads, ROW)[1, 1] = 0
+    _check_range(_fill(c, rows), k3g)
+
+
+@pytest.mark.parametrize("scale", [0.06, -0.06])
+def test_attn_mx8_large_scores(k3g, dev, scale):
+    """As with bf16 pages: scores of +-60, and the order turned round."""
+    Case(dev, 2, 2, 24, 700, [300, 90], seed=4, scale=scale, q_std=20.0).check(k3g)
+
+
+@pytest.mark.parametrize("jump", [0, 20])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attn_mx8_scores_that_grow_token_by_token(k3g, dev, sign, jump):
+    """Every page raises the maximum by about 20 (base e), with latents of one size or of sizes that change by 2^20 from page to page: what was
+    summed before is scaled down again and again, in units that the exponents shift."""
+    c = Case(dev, 1, 1, 24, 64 * 12, [64], seed=70, scale=float(sign), q_std=0.0)
+    c.q[..., :] = 0
+    c.q.reshape(1, 1, 24, ROW)[..., 575] = 0x3F80               # q = 1 on the last rope column: the score is that column of the key
+    rows = normal_bf16(c.g, (c.pages * 64, ROW))
+    rows = k3o.bf16_to_f32(rows.reshape(-1)).reshape(rows.shape).copy()
+    for t in range(64 * 12):
+        rows[_token(c.prefix_table, t), 575] = sign * (20.0 * (t // 64) + 0.25 * (t % 7) - 100)
+        rows[_token(c.prefix_table, t), :LATENT] *= 2.0 ** (jump * (t // 64 % 2))
+    _check_range(_fill(c, rows), k3g)
+
+
 # ---- verification ------------------------------------------------------------------------------------------------------------
 def _probs(g, shape, std=2.5):
     x = g.standard_normal(shape) * std

@@ -414,9 +414,10 @@ int k3g_latent_mx8_gather(const void* cache, const void* block_table, long long 
  * tables' capacity are cut to it.  q [B, S, heads, 576] bf16, q_stride elements (a multiple of 8) from one step to the next; out
  * [B, S, heads, 512] bf16.
  *   - lens[b] < 0: no sequence (a padded batch); its rows of out are left as they were.
- *   - a row that sees no token is zero.  One that sees a NaN, or a score of +infinity, is NaN; a token whose score is -infinity
- *     weighs nothing, but among the tokens that not all steps see (and those in one tile with them) an infinite value makes the
- *     rows that see it NaN.  Rows that do not see it are not touched by it, and what lies behind a page's last token is not used.
+ *   - a row that sees no token is zero.  One that sees a NaN, or a score of +infinity, is NaN.  A token whose score is -infinity
+ *     weighs nothing, but a latent column in which it is infinite is NaN in the outputs (0 times infinity); and among the tokens that
+ *     not all steps see (and those in one tile with them) an infinite value makes the rows that see it NaN.  Rows that do not see it are not
+ *     touched by it, and what lies behind a page's last token is not used.
  *   - MXFP8 pages, with M_j the largest latent magnitude in the 16 tokens (16 i .. 16 i + 15 of a page) that token j lies among: an element below
  *     2^-31 M_j, or below 2^-96, may count as 0; a token's weight p_j may be off by 2^-33 max_i(p_i M_i) / M_j in the outputs (not in the sum of the
  *     weights); a query's latent element below 2^-39 of its row's largest may count as 0.

@@ -78,7 +78,7 @@ struct AttnArgs {
   int2* spans;                       // [row tiles] first and last CTA of each (unwritten where there are no tokens)
   float2* sums;                      // [parts][64] (maximum in log2 units, sum)
   float* parts;                      // [parts][64 groups of 8 columns][64 rows][8]: what a warp writes at a time lies together
-  int B, S, heads, prefix_tiles, seq_tiles, ctas;
+  int B, S, heads, prefix_tiles, seq_tiles;
   float c;                           // |scale| * log2(e), above 0 (scores are compared before they are scaled)
   int flip;                          // the scale is negative
 };
@@ -1054,7 +1054,7 @@ K3G_API int k3g_latent_attn(const void* q, long long q_stride, const void* cache
   AttnArgs a = {(const __nv_bfloat16*)q, q_stride, (const unsigned char*)cache + layer_off * unit, page_stride * unit, pages,
                 (const int*)prefix_table, (const int*)prefix_len, prefix_pages, (const int*)block_table, (const int*)lens, max_pages,
                 (__nv_bfloat16*)out, (int*)ws, (int2*)(ws + sp.spans), (float2*)(ws + sp.sums), (float*)(ws + sp.parts),
-                B, S, heads, (int)((rows + kRows - 1) / kRows), (S * heads + kRows - 1) / kRows, ctas, fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-30f), scale < 0.f};
+                B, S, heads, (int)((rows + kRows - 1) / kRows), (S * heads + kRows - 1) / kRows, fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-30f), scale < 0.f};
   e = k3g_launch_behind(kernel, (unsigned)ctas, kThreads, kSmem, 1, k3g_stream(stream), a);
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   // Few rows mean many parts for each: several teams share them.

@@ -419,6 +419,42 @@ def test_attn_workspace_of_a_larger_batch_serves_a_smaller_one(k3g, dev):
     c.compare(bf16_bits(c.out))
 
 
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("bad", [0x7F80, 0xFF80])
+def test_attn_an_infinite_latent_that_every_step_sees(k3g, dev, own, bad):
+    """An infinity in a latent column, on bf16 pages, in the prefix or among the tokens of a batch without drafts: rows whose score of that token is
+    +infinity are NaN, for the others it weighs nothing, but 0 times the infinity makes that column of their outputs NaN.  Other sequences
+    do not see an own token."""
+    import torch
+    c = Case(dev, 2, 1, 24, 100, [70, 30], mx8=False, seed=80 + own, max_pages=2)
+    table, t = (c.tables[0], 33) if own else (c.prefix_table, 77)
+    at = int(table[t // 64]) * c.stride + c.off + (t % 64) * ROW
+    c.cache[at + 17] = bad
+    c.upload(k3g).call(k3g)
+    torch.cuda.synchronize()
+    got = k3o.bf16_to_f32(bf16_bits(c.out)).astype(np.float64)
+    q17 = k3o.bf16_to_f32(np.ascontiguousarray(c.q)).reshape(c.B, c.S, c.heads, ROW)[..., 17]
+    up = (q17 > 0) == (bad == 0x7F80)
+    seen = np.array([True, not own])[:, None, None]
+    assert (q17 != 0).all() and (up & seen).any() and (~up & seen).any()
+    read = lambda tab, n: _rows_but(c, tab, n, int(table[t // 64]), t % 64)
+    q = k3o.bf16_to_f32(np.ascontiguousarray(c.q)).astype(np.float64).reshape(c.B, c.S, c.heads, ROW)
+    want, spread, ds = attn_oracle(q, read, c.prefix_table, c.prefix, c.tables, c.lens, c.scale)
+    nan = np.isnan(got)
+    assert nan[up & seen].all()
+    assert np.array_equal(nan[~up & seen], np.broadcast_to(np.arange(LATENT) == 17, nan[~up & seen].shape)) and not nan[~(up & seen) & ~seen].any()
+    off = np.abs(np.where(nan, want, got) - want) - attn_tolerance(want, spread, ds)
+    assert np.all(off <= 0)
+
+
+def _rows_but(c, table, n, page, at):
+    rows, held = bf16_rows(c.cache, c.off, c.stride, table, n)
+    for t in range(at, n, 64):
+        if int(table[t // 64]) == page:
+            rows[t], held[t] = 0, False
+    return rows, held
+
+
 # ---- exponents of MXFP8 pages ------------------------------------------------------------------------------------------------
 def _fill(c, rows):
     """The whole cache of an MXFP8 case from rows [pages * 64, 576] of floats."""

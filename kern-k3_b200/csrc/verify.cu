@@ -239,10 +239,13 @@ K3G_API int k3g_verify_draft(const void* target, long long target_stride, const 
   K3G_REQUIRE(S <= kMaxSteps && B <= (1 << 24) && V <= (1 << 30), K3G_ELIMIT);
   if (B == 0) return K3G_OK;
   K3G_REQUIRE(V > 0 && target_stride >= V && (!draft || draft_stride >= V), K3G_ESHAPE);
-  // Blocks per sequence: as many as fit the card in one wave (four blocks of 512 threads on each of 148 SMs), while a block
-  // still has a few thousand elements to read.
+  // Blocks per sequence: where all blocks have an SM to themselves (148), as many as leave each 2048 elements; where they share SMs the blocks of a cluster
+  // wait for one another's, and each needs 16384 to be worth it.  With 1, 2, 4 and 8 blocks a sequence, with q: 1 x 8000 entries 7.9, 6.9, 6.4, 6.4 us;
+  // 1 x 163840 42, 25, 16, 10.5; 64 x 2000 5.6, 6.4, 7.4, 10.7; 64 x 8000 8.3, 7.2, 7.9, 11.2; 80 x 8000 8.4, 8.8, 10.3, 14.6; 64 x 32000 13.8, 11.0, 12.6,
+  // 13.9; 80 x 32000 13.9, 15.8, 18.4, 17.3; 64 x 163840 68, 39, 28.4, 26.4; 80 x 163840 68, 46, 43, 34; 160 x 163840 83, 75, 58, 56; 296 x 163840, which two
+  // blocks each just fill the card with, 87, 81, 86, 92.
   int ranks = kMaxCluster;
-  while (ranks > 1 && ((long long)B * ranks > 592 || V < ranks * 2048)) ranks /= 2;
+  while (ranks > 1 && V < ranks * ((long long)B * ranks <= 148 ? 2048 : 16384)) ranks /= 2;
   const int per = kSegs * 4 * ranks;
   const int slice = (int)(((long long)V + per - 1) / per) * kSegs * 4;
   const bool vec = target_stride % 4 == 0 && (!draft || draft_stride % 4 == 0);

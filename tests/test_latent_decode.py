@@ -644,6 +644,18 @@ def test_verify(k3g, dev, with_probs, B, S, V, stride):
     assert np.array_equal(acc, o_acc) and np.array_equal(tok, o_tok)
 
 
+@pytest.mark.parametrize("B,V", [(74, 4095), (74, 4096), (75, 32767), (75, 32768), (80, 131072), (19, 131071)])
+def test_verify_blocks_per_sequence(k3g, dev, B, V):
+    """On either side of the borders between one, two, four and eight blocks a sequence, and with more clusters than the card holds at once."""
+    g = rng(B + V)
+    target, draft = _probs(g, (B, 2, V)), _probs(g, (B, 1, V))
+    ids, u = g.integers(0, V, (B, 1)), g.random((B, 2), dtype=np.float32)
+    ids[::2, 0] = np.argmax(target[::2, 0], -1)
+    acc, tok = _verify(k3g, dev, target, draft, ids, u)
+    o_acc, o_tok = verify_oracle(target, draft, ids, u)
+    assert 0 < o_acc.sum() < B and np.array_equal(acc, o_acc) and np.array_equal(tok, o_tok)
+
+
 def test_verify_borders(k3g, dev):
     """Exact ties, both ends of the random numbers, drafts of probability 0, equal distributions, empty and spoilt rows."""
     V = 8

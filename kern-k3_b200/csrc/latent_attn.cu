@@ -1057,9 +1057,11 @@ K3G_API int k3g_latent_attn(const void* q, long long q_stride, const void* cache
                 B, S, heads, (int)((rows + kRows - 1) / kRows), (S * heads + kRows - 1) / kRows, fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-30f), scale < 0.f};
   e = k3g_launch_behind(kernel, (unsigned)ctas, kThreads, kSmem, 1, k3g_stream(stream), a);
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
-  // Few rows mean many parts for each: several teams share them.
+  // Few rows mean many parts for each and few blocks: several teams share a row's
+  // parts.  Whole calls with 1, 2 and 4 teams, own 512 tokens and a prefix of 8192: 768 rows 51.8, 44.0, 42.1 us; 1152 rows 58.7, 52.4, 50.9; 1200 rows 58.1, 52.5,
+  // 53.3; 2400 rows 89.1, 85.8, 89.6; 4608 rows 142.8, 142.5, 146.0 (without the prefix 30.2, 30.4, 34.4).
   const int n = (int)rows;
-  e = n <= 1184 ? launch_join<4>(a, ctas, n, k3g_stream(stream)) : n <= 2368 ? launch_join<2>(a, ctas, n, k3g_stream(stream)) : launch_join<1>(a, ctas, n, k3g_stream(stream));
+  e = n <= 8 * sms ? launch_join<4>(a, ctas, n, k3g_stream(stream)) : n <= 24 * sms ? launch_join<2>(a, ctas, n, k3g_stream(stream)) : launch_join<1>(a, ctas, n, k3g_stream(stream));
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   return k3g_launch_status();
 }

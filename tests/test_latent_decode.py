@@ -199,6 +199,11 @@ def test_attn_rows_joined_by_one_two_and_four_teams(k3g, dev, mx8, B, S, heads):
     Case(dev, B, S, heads, 1000, [S + (i * 29) % 150 for i in range(B)], mx8=mx8, seed=31).check(k3g)
 
 
+@pytest.mark.parametrize("B", [148, 149])
+def test_attn_rows_on_either_side_of_one_team(k3g, dev, B):
+    Case(dev, B, 1, 24, 130, [1 + (i * 29) % 150 for i in range(B)], seed=35).check(k3g)
+
+
 def test_attn_many_rows(k3g, dev):
     """More row tiles than SMs, with sequences that begin inside a tile."""
     Case(dev, 150, 3, 24, 130, [3 + (i * 37) % 100 for i in range(150)], seed=3).check(k3g)

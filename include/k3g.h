@@ -413,7 +413,7 @@ int k3g_latent_mx8_gather(const void* cache, const void* block_table, long long 
  * decoding, S > 1 drafted tokens), whose latents are in the cache before the call.  All i32 on the device; lengths beyond the
  * tables' capacity are cut to it.  q [B, S, heads, 576] bf16, q_stride elements (a multiple of 8) from one step to the next; out
  * [B, S, heads, 512] bf16.
- *   - lens[b] < 0: no sequence (a padded batch); its rows of out are left as they were.
+ *   - lens[b] < 0: no sequence (a padded batch); its rows of out are left as they were (its products with the prefix are made all the same).
  *   - a row that sees no token is zero.  One that sees a NaN, or a score of +infinity, is NaN.  A token whose score is -infinity
  *     weighs nothing, but a latent column in which it is infinite is NaN in the outputs (0 times infinity); and among the tokens that
  *     not all steps see (and those in one tile with them) an infinite value makes the rows that see it NaN.  Rows that do not see it are not

@@ -9,8 +9,8 @@
 // two neighbouring lanes (its maximum is one shuffle), codes move as one 16-byte access per lane, and lanes 0..7 move the
 // rope columns.  No shared memory, no block barrier.  One row and no loop: 131072 rows are stored in 39 us (6.1 TB/s, 93% of a
 // copy), with a loop over rows 44, with two or four rows loaded ahead 40 and 41; 65500 rows are read back in 22.5 us (5.3 TB/s:
-// nearly twice as many bytes are written as read), with two rows ahead 24.8.  Launched behind what comes before, 37.5 and 20.4 us.  A few
-// hundred rows take the launch, 5 us.
+// nearly twice as many bytes are written as read), with two rows ahead 24.8.  Launched behind what comes before, 37.2 and 20.4 us (6.4 and
+// 5.8 TB/s); 16383 rows are stored in 5.0 us, 96 in 1.5.
 #include "latent_page.cuh"
 #include "k3g_host.h"
 

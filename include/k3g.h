@@ -419,8 +419,8 @@ int k3g_latent_mx8_gather(const void* cache, const void* block_table, long long 
  *     not all steps see (and those in one tile with them) an infinite value makes the rows that see it NaN.  Rows that do not see it are not
  *     touched by it, and what lies behind a page's last token is not used.
  *   - MXFP8 pages, with M_j the largest latent magnitude in the 16 tokens (16 i .. 16 i + 15 of a page) that token j lies among: an element below
- *     2^-31 M_j, or below 2^-96, may count as 0; a token's weight p_j may be off by 2^-33 max_i(p_i M_i) / M_j in the outputs (not in the sum of the
- *     weights); a query's latent element below 2^-39 of its row's largest may count as 0.
+ *     2^-31 M_j, or below 2^-96, may count as 0; a token's weight p_j may be off by 2^-33 max_i(p_i M_i) / M_j in the outputs, and missing from the sum
+ *     of the weights where p_j M_j is below 2^-130 max_i(p_i M_i) but not 0; a query's latent element below 2^-39 of its row's largest may count as 0.
  *   - prefix_pages = 0 / max_pages = 0: no prefix / no own tokens (the tables, and prefix_len, may be null).
  *   - workspace: 16-byte aligned device memory of k3g_latent_attn_workspace bytes (else K3G_EWORKSPACE), used by one call at a time:
  *     calls that may overlap, and captured graphs that may run together, need one each.  Its content need not be kept.

@@ -38,7 +38,8 @@
 // Types.  bf16 pages are multiplied as bf16.  MXFP8 codes become f16, not bf16: one conversion and one product for two codes, a third of what bf16
 // takes (which has no conversion from E4M3), and the loaders' instructions are what a tile waits for.  f16 has the bits (a code has four), but not the
 // range, so exponents are taken out: of the scales of 16 tokens (but those of blocks of zeros) the largest less kRoom, E (K' = code * 2^(e - E): blocks whose
-// scale is 2^-32 of the largest become 0, others keep what is above 2^-24 of 2^E, 2^-39 of the largest element), of a query row its own (the largest element
+// scale is 2^-32 of the largest become 0, others keep what is above 2^-24 of 2^E, 2^-39 of the largest element; 16 tokens that are all zeros do not move
+// m, and their weights are summed relative to their own maximum), of a query row its own (the largest element
 // is brought to 2^14..2^15; what that costs is below 2^-39 of it).  They come back in f32: S = 2^(E + row) S' + S_rope
 // (the rope columns are multiplied as bf16 into a second accumulator), and P' = 2^(S + E - m), with m the running maximum of S + E, so
 // that P' V' has the weight of P V.  P is rounded because both operands of the matrix instructions are 16 bits; the sums of P stay unrounded in f32.
@@ -62,7 +63,8 @@ constexpr int kSmemQ = 8 * kQChunk, kSmemP = 2 * kQChunk, kSmemK = 9 * kChunk, k
 // half), the rope columns' part of S 320..383 (MXFP8), the queries' rope columns 384..415 (the same on both halves)
 constexpr int kTmemS = 256, kTmemR = 320, kTmemQ = 384;
 constexpr int kRoom = 7;                                     // E is the largest scale's exponent less this: codes reach 448 = 2^8.8, f16 2^16
-constexpr int kLeastE = -80;                                 // sums of 2^-E stay in range (E is 120 at most)
+constexpr int kLeastE = -80, kMostE = 120;                   // sums of 2^-E stay in range
+constexpr int kZeros = kLeastE - 1;                          // 16 tokens that are all zeros: as if their E was the least, and each row's sum finds its own
 constexpr float kLag = 4.f, kTop = 10.f;                     // the long document above 340 us when it was chosen, with a lag of 0 (O rescaled for every new maximum) 359
 constexpr int kPartFloats = kRows * kLatent;                 // a part's outputs; its 64 (maximum, sum) pairs lie in a table of their own
 constexpr int kWaitLimit = 1 << 20, kRing = 4, kReaders = kSoftmax / 32 + 1, kTiles = 2;
@@ -342,10 +344,11 @@ struct Loader {
     if ((token & 63) + 8 * g >= here.tokens) o.u[0] = o.u[1] = o.u[2] = o.u[3] = make_uint4(0u, 0u, 0u, 0u);
     return o;
   }
+  __device__ __forceinline__ static unsigned base_of(unsigned most) { return (unsigned)max((int)most - 1 - kRoom, 127 + kLeastE); }
   // The largest scale byte again, of blocks that are not all zeros: those have byte 127 whatever lies beside them, and where the others' are below it
   // it would take the range from them.  Run only where 127 is the largest byte: latents whose blocks hold magnitudes up to 224 get there through a block
   // of zeros alone.  (From registers: 318 us for the long document, with the look left out 315; in a rolled loop from L2 318.)
-  __device__ __forceinline__ unsigned most_of_blocks() const {
+  __device__ __forceinline__ unsigned base_of_blocks() const {
     unsigned most = 0;
 #pragma unroll
     for (int p = 0; p < 4; ++p)
@@ -357,7 +360,8 @@ struct Loader {
         for (int x = 0; x < 8; ++x) any |= code[p][g].w[x];
         if (byte != 255 && (any & 0x7f7f7f7fu) != 0 && (token & 63) + 8 * g < here.tokens) most = max(most, byte + 1);
       }
-    return __reduce_max_sync(0xffffffffu, most);
+    most = __reduce_max_sync(0xffffffffu, most);
+    return most ? base_of(most) : 127 + kZeros;
   }
   unsigned bad[2];                                           // the thread's tokens have values that are not finite
   __device__ __forceinline__ void put(int p, int g, const Units& o) {
@@ -386,8 +390,7 @@ struct Loader {
         if ((token & 63) + 8 * g < here.tokens) most = max(most, max(m & 0xffffu, m >> 16));
       }
       most = __reduce_max_sync(0xffffffffu, most);
-      if (most == 128) most = most_of_blocks();
-      most = (unsigned)max((int)most - 1 - kRoom, 127 + kLeastE);
+      most = most == 128 ? base_of_blocks() : base_of(most);
     }
     Units u = convert(0, 0, most), v = convert(0, 1, most);
     empty(i, 0);
@@ -629,6 +632,7 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigne
       const int live = min(seen - t * kTile - half * 64, *(volatile int*)&k.tokens[half]) - part * 32;
       unsigned mine = 0;                                     // those with values that are not finite, in tiles that not all rows see all of
       if (s.b >= 0 && a.S > 1 && live > 0) mine = *(volatile unsigned*)&k.poison[i & 1][2 * half + part] & (~0u >> (32 - min(live, 32)));
+      const bool zeros = MX8 && min(ex[0], ex[1]) == kZeros;
       wait(k, k.s_full, i & 1);
       fence_after();
       if (MX8 && t == s.t0) row_scale = __uint_as_float((unsigned)(127 + *(volatile signed char*)&k.row_shift[n & 1][r]) << 23);
@@ -658,20 +662,20 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigne
         for (int j = 0; j < 32; ++j) raw[j] = j < live ? raw[j] : 0xff800000u;
       }
       if (mine) l = NAN;
-      // the row's maximum only where a score is above what P and O are relative to: all four threads of all 32 rows vote
+      // the row's maximum only where a score is above what P and O are relative to (or tokens are all zeros, below): all four threads of all 32 rows vote
       float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < 16; ++j) tops[j >> 2] = max3(tops[j >> 2], __uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1]));
       float top = fmaxf(fmaf(fmaxf(tops[0], tops[1]), a.c, (float)ex[0]), fmaf(fmaxf(tops[2], tops[3]), a.c, (float)ex[1]));
-      if (softmax_vote(rows32, t == s.t0 || top > m + kLag)) {
+      if (softmax_vote(rows32, t == s.t0 || zeros || top > m + kLag)) {
         k.best[2 * part + half][r] = top;
         softmax_barrier(rows32);
         top = fmaxf(fmaxf(k.best[0][r], k.best[1][r]), fmaxf(k.best[2][r], k.best[3][r]));
         if (t == s.t0) {
           m = top;
         } else {                                             // O of these 32 rows catches up with the maximum; the product before this one is done
-          const float best = fmaxf(m, top), f = best == -INFINITY ? 1.f : exp2_fast(m - best);
-          l *= f;
+          const float best = fmaxf(m, top), h = best == -INFINITY ? 1.f : exp2_fast(0.5f * (m - best)), f = h * h;
+          l = l * h * h;                                     // by halves: where E has grown by more than f32's range, the sum has not
           m = best;
 #pragma unroll 1
           for (int c = 0; c < 256; c += 64) {
@@ -683,6 +687,15 @@ __device__ void softmax_tiles(const AttnArgs& a, Control& k, unsigned q, unsigne
             tmem_st32(o + c, v);
           }
           tmem_wait_st();
+        }
+        if (zeros) {                                         // P' does not count there, so the exponentials may be relative to these tokens' own maximum
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            float best = -INFINITY;
+#pragma unroll
+            for (int j = 16 * g; j < 16 * g + 16; j += 2) best = max3(best, __uint_as_float(raw[j]), __uint_as_float(raw[j + 1]));
+            if (ex[g] == kZeros) ex[g] = min(max(__float2int_rd(m - best * a.c), kZeros), kMostE);
+          }
         }
       }
       const float off = kTop - (m == -INFINITY ? 0.f : m);
@@ -954,9 +967,9 @@ __global__ void __launch_bounds__(128 * GROUPS) latent_attn_join_kernel(const __
     float4 v[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) v[x] = __ldcs(reinterpret_cast<const float4*>(a.parts + part * kPartFloats + col + r * 8 + x * 4 * (kRows * 8)));
-    const float top = fmaxf(best, ml.x), off = top == -INFINITY ? 0.f : top, f0 = exp2f(best - off), f = exp2f(ml.x - off);
+    const float top = fmaxf(best, ml.x), off = top == -INFINITY ? 0.f : top, h0 = exp2f(0.5f * (best - off)), h = exp2f(0.5f * (ml.x - off)), f0 = h0 * h0, f = h * h;
     best = top;
-    l = fmaf(ml.y, f, l * f0);
+    l = ml.y * h * h + l * h0 * h0;                          // by halves, as there
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       acc[x].x = fmaf(v[x].x, f, acc[x].x * f0); acc[x].y = fmaf(v[x].y, f, acc[x].y * f0);
@@ -974,9 +987,9 @@ __global__ void __launch_bounds__(128 * GROUPS) latent_attn_join_kernel(const __
 #pragma unroll
     for (int i = 0; i < GROUPS - 1; ++i) {
       const float2 ml = s_sum[i][t];
-      const float top = fmaxf(best, ml.x), off = top == -INFINITY ? 0.f : top, f0 = exp2f(best - off), f = exp2f(ml.x - off);
+      const float top = fmaxf(best, ml.x), off = top == -INFINITY ? 0.f : top, h0 = exp2f(0.5f * (best - off)), h = exp2f(0.5f * (ml.x - off)), f0 = h0 * h0, f = h * h;
       best = top;
-      l = fmaf(ml.y, f, l * f0);
+      l = ml.y * h * h + l * h0 * h0;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float4 v = s_out[i][x][t];

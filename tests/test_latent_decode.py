@@ -500,6 +500,31 @@ def test_attn_mx8_zeros_beside_small_latents(k3g, dev, size, where):
     _fill(c, rows).check(k3g)
 
 
+@pytest.mark.parametrize("where", ["sixteen rows", "rows of another tile", "the first tiles", "all but a few", "all"])
+@pytest.mark.parametrize("size", [0, 40, 60, 115])
+def test_attn_mx8_zeros_beside_large_latents(k3g, dev, size, where):
+    """Tokens that are all zeros weigh what their scores give, however large the others' latents are, and whether they come first or last."""
+    c = Case(dev, 2, 2, 12, 700, [70, 200], seed=46 + size)
+    rows = normal_bf16(c.g, (c.pages * 64, ROW))
+    rows = k3o.bf16_to_f32(rows.reshape(-1)).reshape(rows.shape).copy()
+    rows[:, :LATENT] *= np.float32(2.0 ** size)
+    p = c.prefix_table
+    if where == "sixteen rows":
+        rows[[_token(p, t) for t in range(16, 32)], :LATENT] = 0
+    elif where == "rows of another tile":
+        rows[[_token(p, t) for t in range(256, 600)], :LATENT] = 0
+        rows[[_token(c.tables[1], t) for t in range(128)], :LATENT] = -0.0
+    elif where == "the first tiles":
+        rows[[_token(p, t) for t in range(690)], :LATENT] = 0
+    elif where == "all but a few":
+        keep = [_token(p, 450), _token(c.tables[0], 20), _token(c.tables[1], 180)]
+        rows[np.setdiff1d(np.arange(len(rows)), keep), :LATENT] = 0
+    else:
+        rows[:, :LATENT] = 0
+    _scale_q(c, [2.0 ** -size] * c.heads)
+    _check_range(_fill(c, rows), k3g)
+
+
 @pytest.mark.parametrize("zeros", [False, True])
 def test_attn_mx8_a_nan_scale_over_codes_of_zero(k3g, dev, zeros):
     """Scale byte 255 is NaN whatever it scales, with a block of zeros among the sixteen tokens and without."""

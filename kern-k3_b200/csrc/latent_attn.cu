@@ -558,8 +558,8 @@ __device__ __forceinline__ void fetch_q(const AttnArgs& a, Control& k, const Seg
     for (int i = 0; i < 16; ++i) top = max(top, absmax8(V8{{x[i].x, x[i].y, x[i].z, x[i].w}}));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = (int)(top >> 7);                           // exponent field of the largest element; 0: a row of zeros (or of subnormals), 255: not finite
-    const int shift = e == 0 || e == 255 ? 0 : max(e - 127 - 14, -120);   // q' = q * 2^-shift
+    const int e = (int)(top >> 7);                           // exponent field of the largest element; 0: subnormals or zeros, 255: not finite
+    const int shift = e == 255 ? 0 : max(e - 127 - 14, -120);   // q' = q * 2^-shift
     up = __uint_as_float((unsigned)(127 - shift) << 23);
     if ((tid & 3) == 0) k.row_shift[n & 1][r] = (signed char)shift;
   }

@@ -613,6 +613,18 @@ def test_attn_mx8_query_rows_of_any_size(k3g, dev, size, scale):
     _check_range(_fill(c, rows), k3g)
 
 
+def test_attn_mx8_queries_below_the_normal_numbers(k3g, dev):
+    """Query rows of subnormal bf16 against latents of 2^110: their scores are ordinary ones, with a scale of 2^15."""
+    c = Case(dev, 2, 1, 6, 100, [70, 130], seed=75, scale=2.0 ** 15)
+    rows = normal_bf16(c.g, (c.pages * 64, ROW))
+    rows = k3o.bf16_to_f32(rows.reshape(-1)).reshape(rows.shape).copy()
+    rows[:, :LATENT] *= np.float32(2.0 ** 110)
+    q = c.g.integers(0, 64, c.q.shape).astype(np.uint16) | (c.g.integers(0, 2, c.q.shape) << 15).astype(np.uint16)   # up to 2^-127
+    q.reshape(c.B, c.S, c.heads, ROW)[..., LATENT:] = 0
+    c.q = q
+    _check_range(_fill(c, rows), k3g)
+
+
 @pytest.mark.parametrize("scale", [0.06, -0.06])
 def test_attn_mx8_large_scores(k3g, dev, scale):
     """As with bf16 pages: scores of +-60, and the order turned round."""

@@ -27,13 +27,13 @@
 // 6300 cycles, in two phases that one buffer of 128 tokens keeps apart.  From P to S, 4400: the products, 68 steps of 64 x 128 x 16 that read 6 KB
 // of shared memory each, which is their 48 cycles (3300 in all; at full rate they would be 32, and ncu counts those: 2170 a pair, 31% of the time), and
 // the loaders' conversions and stores between them.  From S to P, 1900: S out of tensor memory, maximum, vote, exponentials.  What the loaders wait for counts: conversions between the stores, polls ahead of the waits and
-// the next tile's place read last brought 321 us down to 298 (for the long document below, before the blocks of zeros were looked for, which costs 1%).  No gain came from more loader warps (16 instead of 8: 346
+// the next tile's place read last brought 321 us down to 298 (for the long document below, before the tokens and blocks of zeros were looked for, which costs 2%).  No gain came from more loader warps (16 instead of 8: 346
 // us instead of 321), from P V in products of 256 columns, which read less but free the chunks later (349 instead of 339), from one
 // accumulator for latent and rope columns (315 instead of 309), or from the rope columns' product before the last pair of chunks (308
 // instead of 303).  A call's start, the parts' way out and the join take 17 us beside the pairs.
-// Measured: 8 x 96 rows against 131072 MXFP8 tokens 304 us (319 in a long run with other inputs every time: 686 TFLOP/s, 42% of a dense bf16
-// product), 48 x 4 x 24 rows against 16384 and their own 512 252 us, 32 x 24 rows against 8229 and 1024 42 us, 64 x 12 rows against
-// their own 4096 42 us (2.1 TB/s), 16 x 2 x 48 rows against bf16 pages 48 us (53 with the next tile asked for before this one was copied), one sequence of 500 tokens 12.9 us.
+// Measured: 8 x 96 rows against 131072 MXFP8 tokens 305 us (319 in a long run with other inputs every time: 686 TFLOP/s, 42% of a dense bf16
+// product), 48 x 4 x 24 rows against 16384 and their own 512 252 us, 32 x 24 rows against 8229 and 1024 43 us, 64 x 12 rows against
+// their own 4096 42 us (2.1 TB/s), 16 x 2 x 48 rows against bf16 pages 48 us (53 with the next tile asked for before this one was copied), one sequence of 500 tokens 12.5 us.
 //
 // Types.  bf16 pages are multiplied as bf16.  MXFP8 codes become f16, not bf16: one conversion and one product for two codes, a third of what bf16
 // takes (which has no conversion from E4M3), and the loaders' instructions are what a tile waits for.  f16 has the bits (a code has four), but not the

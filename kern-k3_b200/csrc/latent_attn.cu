@@ -26,8 +26,9 @@
 // What bounds it.  By the formulas the cache's bytes with few rows, the tensor cores with many (640 flops a byte for 64 rows).  A pair takes
 // 6300 cycles, in two phases that one buffer of 128 tokens keeps apart.  From P to S, 4400: the products, 68 steps of 64 x 128 x 16 that read 6 KB
 // of shared memory each, which is their 48 cycles (3300 in all; at full rate they would be 32, and ncu counts those: 2170 a pair, 31% of the time), and
-// the loaders' conversions and stores between them.  From S to P, 1900: S out of tensor memory, maximum, vote, exponentials.  What the loaders wait for counts: conversions between the stores, polls ahead of the waits and
-// the next tile's place read last brought 321 us down to 298 (for the long document below, before the tokens and blocks of zeros were looked for, which costs 2%).  No gain came from more loader warps (16 instead of 8: 346
+// the loaders' conversions and stores between them.  From S to P, 1900: S out of tensor memory, maximum, vote, exponentials.  What the loaders wait for
+// counts: conversions between the stores, polls ahead of the waits and the next tile's place read last brought 321 us down to 298 (for the long document
+// below, before blocks and tokens of zeros were looked for, which costs 2%).  No gain came from more loader warps (16 instead of 8: 346
 // us instead of 321), from P V in products of 256 columns, which read less but free the chunks later (349 instead of 339), from one
 // accumulator for latent and rope columns (315 instead of 309), or from the rope columns' product before the last pair of chunks (308
 // instead of 303).  A call's start, the parts' way out and the join take 17 us beside the pairs.
@@ -969,7 +970,7 @@ __global__ void __launch_bounds__(128 * GROUPS) latent_attn_join_kernel(const __
     for (int x = 0; x < 4; ++x) v[x] = __ldcs(reinterpret_cast<const float4*>(a.parts + part * kPartFloats + col + r * 8 + x * 4 * (kRows * 8)));
     const float top = fmaxf(best, ml.x), off = top == -INFINITY ? 0.f : top, h0 = exp2f(0.5f * (best - off)), h = exp2f(0.5f * (ml.x - off)), f0 = h0 * h0, f = h * h;
     best = top;
-    l = ml.y * h * h + l * h0 * h0;                          // by halves, as there
+    l = ml.y * h * h + l * h0 * h0;                          // by halves: maxima of S + E may lie further apart than f32's exponents, sums do not
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       acc[x].x = fmaf(v[x].x, f, acc[x].x * f0); acc[x].y = fmaf(v[x].y, f, acc[x].y * f0);
@@ -1070,8 +1071,7 @@ K3G_API int k3g_latent_attn(const void* q, long long q_stride, const void* cache
                 B, S, heads, (int)((rows + kRows - 1) / kRows), (S * heads + kRows - 1) / kRows, fmaxf(fabsf(scale) * 1.44269504088896341f, 1e-30f), scale < 0.f};
   e = k3g_launch_behind(kernel, (unsigned)ctas, kThreads, kSmem, 1, k3g_stream(stream), a);
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
-  // Few rows mean many parts for each and few blocks: several teams share a row's
-  // parts.  Whole calls with 1, 2 and 4 teams, own 512 tokens and a prefix of 8192: 768 rows 51.8, 44.0, 42.1 us; 1152 rows 58.7, 52.4, 50.9; 1200 rows 58.1, 52.5,
+  // Few rows mean many parts for each and few blocks: several teams share a row's parts.  Whole calls with 1, 2 and 4 teams, own 512 tokens and a prefix of 8192: 768 rows 51.8, 44.0, 42.1 us; 1152 rows 58.7, 52.4, 50.9; 1200 rows 58.1, 52.5,
   // 53.3; 2400 rows 89.1, 85.8, 89.6; 4608 rows 142.8, 142.5, 146.0 (without the prefix 30.2, 30.4, 34.4).
   const int n = (int)rows;
   e = n <= 8 * sms ? launch_join<4>(a, ctas, n, k3g_stream(stream)) : n <= 24 * sms ? launch_join<2>(a, ctas, n, k3g_stream(stream)) : launch_join<1>(a, ctas, n, k3g_stream(stream));

@@ -421,10 +421,11 @@ int k3g_latent_mx8_gather(const void* cache, const void* block_table, long long 
  *   - MXFP8 pages, with M_j the largest latent magnitude in the 16 tokens (16 i .. 16 i + 15 of a page) that token j lies among: an element below
  *     2^-31 M_j, or below 2^-96, may count as 0; a token's weight p_j may be off by 2^-33 max_i(p_i M_i) / M_j in the outputs, and missing from the sum
  *     of the weights where p_j M_j is below 2^-130 max_i(p_i M_i) but not 0; a query's latent element below 2^-39 of its row's largest may count as 0.
+ *     A row's scores are made with a factor of its largest latent element times M_j: where that product reaches 2^156 they may be infinite or NaN.
  *   - prefix_pages = 0 / max_pages = 0: no prefix / no own tokens (the tables, and prefix_len, may be null).
  *   - workspace: 16-byte aligned device memory of k3g_latent_attn_workspace bytes (else K3G_EWORKSPACE), used by one call at a time:
  *     calls that may overlap, and captured graphs that may run together, need one each.  Its content need not be kept.
- * B <= 4096, S * heads <= 32768, prefix_pages and max_pages <= 2^20 (K3G_ELIMIT); scale finite (K3G_ERANGE). */
+ * B <= 4096, S * heads <= 32768, prefix_pages and max_pages <= 2^20 (K3G_ELIMIT); scale finite (K3G_ERANGE), a magnitude below 7e-31 counts as that. */
 int k3g_latent_attn(const void* q, long long q_stride, const void* cache, int cache_mx8, long long layer_off, long long page_stride,
                     long long pages, const void* prefix_table, const void* prefix_len, int prefix_pages, const void* block_table,
                     const void* lens, int max_pages, void* out, void* workspace, long long workspace_bytes, int B, int S, int heads,
